@@ -1,4 +1,4 @@
-"""Build libtaco_env.so (the HIP product library) in-tree for gfx950.
+"""Build libtaco_env.so and libtaco_sequence.so (the HIP product libraries) in-tree for gfx950.
 
     python -m taco_amd.build [--force] [--test-hooks]
 
@@ -34,12 +34,22 @@ FLAGS = ["--offload-arch=gfx950", "-O3", "-std=c++17", "-fPIC", "-shared", "-ffp
          "-mllvm", "-amdgpu-kernarg-preload-count=11", "-Wall", "-Wno-unused-function"]
 
 
-def source_hash():
+# libtaco_sequence.so: the sequence kernels (include/taco_sequence.h), a library of their own -- one object per source, compiled side by side.  Fused
+# multiply-adds are the compiler's choice here (no bit contract with a CPU restatement); no packed float32 arithmetic.
+LIB_SEQ = os.path.join(HERE, "libtaco_sequence.so")
+SEQ_SOURCES = ["seq_common.hip", "seq_attention.hip", "seq_attention_grad.hip", "seq_attention_step.hip", "seq_linear.hip"]
+SEQ_DEPS = SEQ_SOURCES + ["seq_core.hpp", "seq_host.hpp", "seq_attention.hpp", "seq_attention_host.hpp", "seq_attention_step.hpp", "seq_pages.hpp", "seq_linear.hpp",
+                          os.path.join("..", "..", "include", "taco_sequence.h")]
+SEQ_FLAGS = ["--offload-arch=gfx950", "-O3", "-std=c++17", "-fPIC", "-fvisibility=hidden", "-fno-exceptions", "-fno-strict-aliasing", "-fno-slp-vectorize",
+             "-Xclang", "-target-feature", "-Xclang", "-packed-fp32-ops", "-Wall", "-Wno-unused-function"]
+
+
+def source_hash(deps=DEPS, flags=FLAGS):
     h = hashlib.sha256()
-    for d in DEPS:
+    for d in deps:
         with open(os.path.join(CSRC, d), "rb") as f:
             h.update(f.read())
-    h.update(" ".join(FLAGS).encode())
+    h.update(" ".join(flags).encode())
     return h.hexdigest()[:16]
 
 
@@ -80,5 +90,37 @@ def build(force=False, verbose=False, test_hooks=False):
     return out
 
 
+def sequence_hash():
+    return source_hash(SEQ_DEPS, SEQ_FLAGS)
+
+
+def build_sequence(force=False, verbose=False):
+    if not force and embedded_hash(LIB_SEQ) == sequence_hash():
+        return LIB_SEQ
+    with open(os.path.join(HERE, ".build.lock"), "w") as lock:
+        fcntl.flock(lock, fcntl.LOCK_EX)
+        if not force and embedded_hash(LIB_SEQ) == sequence_hash():
+            return LIB_SEQ
+        tag = f"{LIB_SEQ}.{os.getpid()}"
+        objs = [f"{tag}.{s}.o.tmp" for s in SEQ_SOURCES]
+        cmds = [[HIPCC] + SEQ_FLAGS + [f'-DTACO_SOURCE_HASH="{sequence_hash()}"', "-c", os.path.join(CSRC, s), "-o", o] for s, o in zip(SEQ_SOURCES, objs)]
+        link = [HIPCC, "--offload-arch=gfx950", "-shared", "-o", f"{tag}.tmp"] + objs
+        try:
+            if verbose:
+                print("\n".join(" ".join(c) for c in cmds + [link]))
+            running = [subprocess.Popen(c, cwd=CSRC) for c in cmds]
+            for r, c in [(p.wait(), c) for p, c in zip(running, cmds)]:
+                if r:
+                    raise subprocess.CalledProcessError(r, c)
+            subprocess.check_call(link, cwd=CSRC)
+            os.replace(f"{tag}.tmp", LIB_SEQ)
+        finally:
+            for f in objs + [f"{tag}.tmp"]:
+                if os.path.exists(f):
+                    os.remove(f)
+    return LIB_SEQ
+
+
 if __name__ == "__main__":
+    print(build_sequence(force="--force" in sys.argv, verbose=True))
     print(build(force="--force" in sys.argv, verbose=True, test_hooks="--test-hooks" in sys.argv))

@@ -1,0 +1,258 @@
+// What the sequence kernels share: element types, 32x32 matrix tiles, swizzled LDS tiles, bounds-checked loads.
+//
+// Every product runs on 32x32 MFMAs with 16 values of the contraction per step.  Lane l = 32 h + r of the A operand holds row r and the contraction's
+// slots 8 h + j, j < 8; B the same for its columns; register i of the result is row 8 (i / 4) + 4 h + i % 4 of column r.  Two facts carry all kernels:
+//  * a contraction may be permuted as long as A and B agree.  The result of one product (columns = lane) is therefore the B (or A) operand of the
+//    next one as it stands: slot (h, j) of step s is row 16 s + 8 (j / 4) + 4 h + j % 4, "permuted order" below.  Scores never leave the registers.
+//  * float32 runs through the same fragments: eight 32x32x2 MFMAs take element j of both operands in turn.
+#pragma once
+#include <hip/hip_runtime.h>
+#include <stdint.h>
+
+namespace seq {
+
+typedef float f32x4 __attribute__((ext_vector_type(4)));
+typedef float f32x8 __attribute__((ext_vector_type(8)));
+typedef float f32x16 __attribute__((ext_vector_type(16)));
+typedef _Float16 f16x8 __attribute__((ext_vector_type(8)));
+typedef __bf16 bf16x8 __attribute__((ext_vector_type(8)));
+typedef short s16x4 __attribute__((ext_vector_type(4)));
+typedef short s16x8 __attribute__((ext_vector_type(8)));
+typedef uint32_t u32x4 __attribute__((ext_vector_type(4)));
+typedef __bf16 bf16;
+typedef _Float16 f16;
+
+template <typename T> struct Frag;
+template <> struct Frag<float> { typedef f32x8 type; };
+template <> struct Frag<f16> { typedef f16x8 type; };
+template <> struct Frag<bf16> { typedef bf16x8 type; };
+template <typename T> using frag = typename Frag<T>::type;
+
+__device__ __forceinline__ f32x16 mma(bf16x8 a, bf16x8 b, f32x16 c) { return __builtin_amdgcn_mfma_f32_32x32x16_bf16(a, b, c, 0, 0, 0); }
+__device__ __forceinline__ f32x16 mma(f16x8 a, f16x8 b, f32x16 c) { return __builtin_amdgcn_mfma_f32_32x32x16_f16(a, b, c, 0, 0, 0); }
+__device__ __forceinline__ f32x16 mma(f32x8 a, f32x8 b, f32x16 c) {
+#pragma unroll
+    for (int j = 0; j < 8; ++j) c = __builtin_amdgcn_mfma_f32_32x32x2f32(a[j], b[j], c, 0, 0, 0);
+    return c;
+}
+
+// row (of a product's result) that register i of half h holds; also the permuted order of a contraction, i = 8 (step % 2) + j
+__device__ __forceinline__ int row_of(int i, int h) { return 8 * (i / 4) + 4 * h + i % 4; }
+
+// registers 8 s .. 8 s + 7 of a result as an operand in permuted order: rounded to nearest even, once
+template <typename T> __device__ __forceinline__ frag<T> to_frag(const f32x16 &x, int s) {
+    frag<T> f;
+#pragma unroll
+    for (int j = 0; j < 8; ++j) f[j] = (T)x[8 * s + j];
+    return f;
+}
+
+template <int N> __device__ __forceinline__ void clear(f32x16 (&x)[N]) {
+#pragma unroll
+    for (int n = 0; n < N; ++n)
+#pragma unroll
+        for (int i = 0; i < 16; ++i) x[n][i] = 0.f;
+}
+
+__device__ __forceinline__ float other_half(float x) { return __shfl_xor(x, 32); }
+__device__ __forceinline__ float exp2_(float x) { return __builtin_amdgcn_exp2f(x); }
+__device__ __forceinline__ float log2_(float x) { return __builtin_amdgcn_logf(x); }
+constexpr float LOG2E = 1.4426950408889634f, LN2 = 0.6931471805599453f;
+
+// ---- LDS tiles: rows of DP elements (the head dimension padded with zeros to 32, 64 or 128), 16-byte chunks exchanged inside each row by an XOR that
+// depends on the row.  256 bytes are one turn of the 64 banks.  A row-wise read (32 rows, the same chunk) wants 16 neighbouring rows in 16 different
+// chunk positions; a column-wise read (4 neighbouring rows, 64 bytes each) wants the four rows in different quarters.  flip() gives both.
+template <typename T, int DP> struct Tile {
+    static constexpr int NC = DP * (int)sizeof(T) / 16;         // chunks of a row
+    static constexpr int CE = 16 / (int)sizeof(T);              // elements of a chunk
+    static constexpr int ROW = NC * 16;                         // bytes of a row
+    static __device__ __forceinline__ int flip(int r) {
+        if (NC == 4) return (r >> 2) & 3;
+        if (NC == 8) return ((r >> 1) & 1) << 2 | ((r >> 2) & 3);
+        return (r & 3) << 2 | ((r >> 2) & 3);
+    }
+    static __device__ __forceinline__ int at(int r, int c) { return r * ROW + ((c ^ flip(r)) << 4); }
+    static __device__ __forceinline__ void put(char *lds, int r, int c, u32x4 x) { *(u32x4 *)(lds + at(r, c)) = x; }
+    static __device__ __forceinline__ T get(const char *lds, int r, int d) { return *(const T *)(lds + at(r, d / CE) + (d % CE) * (int)sizeof(T)); }
+
+    // operand whose lane is a row of the tile (row0 + l % 32), contraction over the columns 16 s + 8 h + j
+    static __device__ __forceinline__ frag<T> rows(const char *lds, int row0, int s, int lane) {
+        int r = row0 + (lane & 31), h = lane >> 5;
+        if constexpr (sizeof(T) == 2) {
+            return *(const frag<T> *)(lds + at(r, 2 * s + h));
+        } else {
+            f32x4 a = *(const f32x4 *)(lds + at(r, 4 * s + 2 * h)), b = *(const f32x4 *)(lds + at(r, 4 * s + 2 * h + 1));
+            return f32x8{a[0], a[1], a[2], a[3], b[0], b[1], b[2], b[3]};
+        }
+    }
+    // the same with the columns col0 + (permuted order): the partner of a result used as an operand
+    static __device__ __forceinline__ frag<T> rows_permuted(const char *lds, int row0, int col0, int lane) {
+        int r = row0 + (lane & 31), h = lane >> 5;
+        if constexpr (sizeof(T) == 2) {
+            s16x4 a = *(const s16x4 *)(lds + at(r, col0 / 8) + 8 * h), b = *(const s16x4 *)(lds + at(r, col0 / 8 + 1) + 8 * h);
+            return __builtin_bit_cast(frag<T>, __builtin_shufflevector(a, b, 0, 1, 2, 3, 4, 5, 6, 7));
+        } else {
+            f32x4 a = *(const f32x4 *)(lds + at(r, col0 / 4 + h)), b = *(const f32x4 *)(lds + at(r, col0 / 4 + 2 + h));
+            return f32x8{a[0], a[1], a[2], a[3], b[0], b[1], b[2], b[3]};
+        }
+    }
+    // operand whose lane is a column of the tile (col0 + l % 32), contraction over the rows row0 + (permuted order).  16 bit: the transposing LDS
+    // read: 16 lanes name four rows of 16 columns, 8 bytes each, and receive a column of four.  All 64 lanes have to be active.
+    static __device__ __forceinline__ frag<T> cols(const char *lds, int row0, int col0, int lane) {
+        int h = lane >> 5;
+        if constexpr (sizeof(T) == 2) {
+            typedef s16x4 __attribute__((address_space(3))) *lds4;
+            int i = lane & 15, r = row0 + 4 * h + (i >> 2), c = col0 / 8 + 2 * ((lane >> 4) & 1) + ((i & 3) >> 1), b = (i & 1) * 8;
+            s16x4 x = __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds4)(lds + at(r, c) + b));
+            s16x4 y = __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds4)(lds + at(r + 8, c) + b));
+            return __builtin_bit_cast(frag<T>, __builtin_shufflevector(x, y, 0, 1, 2, 3, 4, 5, 6, 7));
+        } else {
+            f32x8 f;
+            int d = col0 + (lane & 31);
+#pragma unroll
+            for (int j = 0; j < 8; ++j) f[j] = get(lds, row0 + row_of(j, h), d);
+            return f;
+        }
+    }
+    // does any element of rows [row0, row0 + n) differ from a finite number?  (wave-uniform answer; every lane takes chunks in turn)
+    static __device__ __forceinline__ bool any_nonfinite(const char *lds, int row0, int n, int lane) {
+        bool bad = false;
+        for (int e = lane; e < n * NC; e += 64) {
+            u32x4 x = *(const u32x4 *)(lds + at(row0 + e / NC, e % NC));
+#pragma unroll
+            for (int i = 0; i < 4; ++i) {
+                if constexpr (sizeof(T) == 4) bad |= (x[i] & 0x7f800000u) == 0x7f800000u;
+                else {
+                    constexpr uint32_t m = __is_same(T, f16) ? 0x7c00u : 0x7f80u;
+                    bad |= (x[i] & m) == m || (x[i] & (m << 16)) == (m << 16);
+                }
+            }
+        }
+        return __any(bad);
+    }
+};
+
+// ---- Global memory.  A buffer descriptor covers the rows of one tile that exist; what lies outside reads as zero, so no lane branches and padding rows and
+// padding columns cost nothing.  The base is 64 bits and moves with the tile, offsets inside it are 32.
+typedef __amdgpu_buffer_rsrc_t rsrc;
+__device__ __forceinline__ rsrc rows_of(const void *base, int rows, uint32_t stride_bytes, uint32_t row_bytes) {
+    uint32_t n = rows > 0 ? (uint32_t)(rows - 1) * stride_bytes + row_bytes : 0u;
+    return __builtin_amdgcn_make_buffer_rsrc((void *)base, 0, n, 0x00020000);
+}
+__device__ __forceinline__ u32x4 load16(rsrc r, uint32_t off) { return __builtin_bit_cast(u32x4, __builtin_amdgcn_raw_buffer_load_b128(r, off, 0, 0)); }
+constexpr uint32_t OUTSIDE = 0x80000000u;      // an offset no descriptor reaches (tiles stay below 2 GiB)
+
+// a tile of ROWS rows in the registers of NT threads, on its way from global memory to LDS
+template <typename T, int DP, int ROWS, int NT> struct Staged {
+    typedef Tile<T, DP> tile;
+    static constexpr int N = ROWS * tile::NC / NT;
+    static_assert(ROWS * tile::NC % NT == 0, "whole chunks per thread");
+    u32x4 x[N];
+    __device__ __forceinline__ void load(rsrc r, uint32_t stride_bytes, int d, int t) {
+#pragma unroll
+        for (int i = 0; i < N; ++i) {
+            int e = i * NT + t, row = e / tile::NC, c = e % tile::NC;
+            x[i] = load16(r, c * tile::CE < d ? row * stride_bytes + c * 16 : OUTSIDE);
+        }
+    }
+    // row j of the tile is row last - j of the descriptor (a sequence read backwards); negative rows wrap to offsets outside
+    __device__ __forceinline__ void load_reversed(rsrc r, uint32_t stride_bytes, int d, int last, int t) {
+#pragma unroll
+        for (int i = 0; i < N; ++i) {
+            int e = i * NT + t, row = last - e / tile::NC, c = e % tile::NC;
+            x[i] = load16(r, c * tile::CE < d && row >= 0 ? row * stride_bytes + c * 16 : OUTSIDE);
+        }
+    }
+    __device__ __forceinline__ void put(char *lds, int t) {
+#pragma unroll
+        for (int i = 0; i < N; ++i) {
+            int e = i * NT + t;
+            tile::put(lds, e / tile::NC, e % tile::NC, x[i]);
+        }
+    }
+};
+
+// operand whose lane is a row of global memory (row0 + l % 32), contraction over the columns 16 s + 8 h + j
+template <typename T> __device__ __forceinline__ frag<T> rows_global(rsrc r, uint32_t stride_bytes, int d, int row0, int s, int lane) {
+    uint32_t off = (row0 + (lane & 31)) * stride_bytes;
+    int c = 16 * s + 8 * (lane >> 5);
+    u32x4 a = load16(r, c < d ? off + c * (int)sizeof(T) : OUTSIDE);
+    if constexpr (sizeof(T) == 2) return __builtin_bit_cast(frag<T>, a);
+    else {
+        u32x4 b = load16(r, c < d ? off + c * 4 + 16 : OUTSIDE);
+        return __builtin_bit_cast(f32x8, __builtin_shufflevector(a, b, 0, 1, 2, 3, 4, 5, 6, 7));
+    }
+}
+
+// four neighbouring elements of a row, rounded to T
+template <typename T> __device__ __forceinline__ void store4(T *p, float a, float b, float c, float d) {
+    if constexpr (sizeof(T) == 4) *(f32x4 *)p = f32x4{a, b, c, d};
+    else {
+        typedef T t4 __attribute__((ext_vector_type(4)));
+        *(t4 *)p = t4{(T)a, (T)b, (T)c, (T)d};
+    }
+}
+
+// acc[db] (rows = dimension, column = this lane's row) * f -> a row of global memory
+template <typename T, int DB> __device__ __forceinline__ void store_row(T *row, const f32x16 (&acc)[DB], float f, int d, int lane) {
+    int h = lane >> 5;
+#pragma unroll
+    for (int b = 0; b < DB; ++b)
+#pragma unroll
+        for (int i = 0; i < 16; i += 4) {
+            int c = 32 * b + 8 * (i / 4) + 4 * h;
+            if (c < d) store4(row + c, acc[b][i] * f, acc[b][i + 1] * f, acc[b][i + 2] * f, acc[b][i + 3] * f);
+        }
+}
+
+// acc[dim][lane's column] += sum over the 32 rows from row0 of X[row][dim] * w[row][column], where rows that are hidden from a column hold NaN or infinities:
+// their w is 0, but a plain matrix product makes NaN of 0 * NaN.  The finite part goes through the product as it is.  What is not finite is counted over
+// the rows a column sees, apart for each sign of the term (a NaN, or a weight of 0, counts for both), and joins as +inf, -inf or their sum, NaN.
+// Runs only where something not finite turned up.
+template <typename T> __device__ __forceinline__ frag<T> part_of(frag<T> f, int which) {      // 0: what is finite; 1: marks of +inf and NaN; 2: of -inf and NaN
+#pragma unroll
+    for (int j = 0; j < 8; ++j) {
+        float x = (float)f[j];
+        bool fin = __builtin_fabsf(x) < __builtin_inff();
+        f[j] = which == 0 ? (fin ? f[j] : (T)0.f) : (T)(!fin && !(which == 1 ? x < 0.f : x > 0.f) ? 1.f : 0.f);
+    }
+    return f;
+}
+template <typename T, int DP, int NB, typename F>
+__device__ __forceinline__ void accumulate_seen(const char *lds, int row0, int col0, const f32x16 &w, F seen, f32x16 (&acc)[NB], int lane) {
+    frag<T> f[2], up[2], down[2];
+#pragma unroll
+    for (int s = 0; s < 2; ++s) {
+        f[s] = to_frag<T>(w, s);
+#pragma unroll
+        for (int j = 0; j < 8; ++j) {
+            bool v = seen(row_of(8 * s + j, lane >> 5));
+            up[s][j] = (T)(v && (float)f[s][j] >= 0.f ? 1.f : 0.f);
+            down[s][j] = (T)(v && (float)f[s][j] <= 0.f ? 1.f : 0.f);
+        }
+    }
+#pragma unroll
+    for (int b = 0; b < NB; ++b) {
+        f32x16 n[2];
+        clear(n);
+#pragma unroll
+        for (int s = 0; s < 2; ++s) {
+            frag<T> x = Tile<T, DP>::cols(lds, row0 + 16 * s, col0 + 32 * b, lane), p = part_of<T>(x, 1), m = part_of<T>(x, 2);
+            acc[b] = mma(part_of<T>(x, 0), f[s], acc[b]);
+            n[0] = mma(m, down[s], mma(p, up[s], n[0]));
+            n[1] = mma(m, up[s], mma(p, down[s], n[1]));
+        }
+#pragma unroll
+        for (int i = 0; i < 16; ++i) acc[b][i] += (n[0][i] > 0.f ? __builtin_inff() : 0.f) + (n[1][i] > 0.f ? -__builtin_inff() : 0.f);
+    }
+}
+template <int N> __device__ __forceinline__ bool any_nan(const f32x16 (&x)[N]) {
+    bool bad = false;
+#pragma unroll
+    for (int n = 0; n < N; ++n)
+#pragma unroll
+        for (int i = 0; i < 16; ++i) bad |= x[n][i] != x[n][i];
+    return __any(bad);
+}
+
+}  // namespace seq

@@ -23,6 +23,7 @@ PyTorch only owns the memory.  There is no torch fallback for the arithmetic.
 import ctypes as C
 import math
 
+import numpy as np
 import torch
 
 from . import _lib
@@ -186,6 +187,17 @@ class RolloutBuffer:
     def time_outs(self):
         """[H, N] uint8: extras["time_outs"] of every step of the last run()"""
         return self._timeouts
+
+    def episodes(self):
+        """The rollout's episodes as packed sequences (taco_amd.sequence.Packed) for the sequence operators: env after env, each env's `step` stored steps cut behind
+        every done flag (an episode that was already under way, or goes on, is cut at the rollout's ends).  Tokens in that order: x [step, N, ...] ->
+        x.transpose(0, 1).reshape(step * N, ...).  BLOCKS (reads the done flags)."""
+        from .sequence import Packed
+        ends = self.done_buf[:self.step, :, 0].cpu().numpy().T != 0
+        if self.step:
+            ends[:, -1] = True
+        at = np.flatnonzero(ends) + 1
+        return Packed(np.diff(at, prepend=0), self.device)
 
     def add_timeout_bootstrap(self, t, env_ids, time_out_value):
         """rewards_augmented[truncated] += gamma * V(s_t)  (ppo_asymmetry.py:320-324) on the stored reward of step t."""

@@ -1,0 +1,289 @@
+"""The sequence operators without a GPU: the C ABI of libtaco_sequence.so, what the host layer and the entry points refuse, the work lists, and the paged cache's index
+arithmetic compiled for the host."""
+import ctypes as C
+import os
+import re
+import subprocess
+
+import numpy as np
+import pytest
+import torch
+
+from taco_amd import _lib, sequence
+
+ROOT = os.path.dirname(os.path.dirname(os.path.abspath(__file__)))
+HEADER = os.path.join(ROOT, "include", "taco_sequence.h")
+
+
+@pytest.fixture(scope="module")
+def lib():
+    return sequence.load()
+
+
+def test_header_library_and_binding_agree(lib):
+    txt = re.sub(r"/\*.*?\*/", "", open(HEADER).read(), flags=re.S)
+    names = sorted(set(re.findall(r"\b(taco_[a-z_]+)\s*\(", txt)))
+    assert names == sorted(sequence.EXPORTS)
+    for n in names:
+        assert hasattr(lib, n)
+    from taco_amd import build
+    assert lib.taco_sequence_source_hash().decode() == build.sequence_hash() == build.embedded_hash(build.LIB_SEQ)
+    syms = [line.split()[-1] for line in subprocess.check_output(["nm", "-D", "--defined-only", build.LIB_SEQ]).decode().splitlines()]
+    assert sorted(s for s in syms if s.startswith("taco_")) == names
+    assert "getenv" not in subprocess.check_output(["nm", "-D", build.LIB_SEQ]).decode()
+
+
+def test_struct_layouts(tmp_path):
+    structs = {"taco_seq_tensor": sequence.Tensor, "taco_attention_args": sequence.AttentionArgs, "taco_attention_step_args": sequence.AttentionStepArgs,
+               "taco_linear_attention_args": sequence.LinearArgs, "taco_linear_attention_step_args": sequence.LinearStepArgs}
+    lines = [f'printf("%zu\\n", sizeof({n}));' + "".join(f'printf("%zu\\n", offsetof({n}, {f[0]}));' for f in t._fields_) for n, t in structs.items()]
+    src = tmp_path / "t.c"
+    src.write_text('#include <stdio.h>\n#include "taco_sequence.h"\nint main(void) {' + "".join(lines) + "return 0; }")
+    subprocess.check_call(["gcc", "-Wall", "-Werror", "-I", os.path.join(ROOT, "include"), "-o", str(tmp_path / "t"), str(src)])
+    got = [int(x) for x in subprocess.check_output([str(tmp_path / "t")]).split()]
+    want = []
+    for t in structs.values():
+        want += [C.sizeof(t)] + [getattr(t, f[0]).offset for f in t._fields_]
+    assert got == want
+
+
+def tensor(p=1 << 20, ts=64, hs=32):
+    return sequence.Tensor(p, ts, hs)
+
+
+def attention_args(**kw):
+    a = sequence.AttentionArgs(tensor(), tensor(), tensor(), tensor(), 1 << 20, 1 << 20, None, 1, 128, 2, 2, 32, 0, 1, 1.0, tensor(), tensor(), tensor(), tensor(), 1 << 20)
+    for k, v in kw.items():
+        setattr(a, k, v)
+    return a
+
+
+def step_args(**kw):
+    a = sequence.AttentionStepArgs(tensor(), tensor(), tensor(), tensor(), 1 << 20, 1 << 20, 1024, 64, 32, 1024, 64, 32, 1 << 20, 4, 1 << 20, 2, 4, 8, 16, 2, 2, 32, 0, 1.0, None, 0)
+    for k, v in kw.items():
+        setattr(a, k, v)
+    return a
+
+
+def linear_args(**kw):
+    a = sequence.LinearArgs(tensor(), tensor(), tensor(), tensor(), 1 << 20, None, None, 1 << 20, 1 << 20, 2, 2, 2, 32, 0, 1.0, None, 0, tensor(), tensor(), tensor(), tensor(), None, None)
+    for k, v in kw.items():
+        setattr(a, k, v)
+    return a
+
+
+def linear_step_args(**kw):
+    a = sequence.LinearStepArgs(tensor(), tensor(), tensor(), tensor(), 1 << 20, 1 << 20, None, 0, 2, 2, 32, 0, 1.0)
+    for k, v in kw.items():
+        setattr(a, k, v)
+    return a
+
+
+BAD_TENSORS = [tensor(p=None), tensor(p=(1 << 20) + 8), tensor(ts=30), tensor(ts=66), tensor(hs=-32), tensor(hs=34), tensor(ts=1 << 22)]
+
+
+@pytest.mark.parametrize("name,make,bad", [
+    ("taco_attention", attention_args, [dict(dim=12), dict(dim=0), dict(dim=136), dict(dtype=3), dict(heads=3), dict(kv_heads=0), dict(scale=0.0), dict(scale=float("nan")),
+                                        dict(scale=float("inf")), dict(tile_rows=64), dict(n_tiles=-1), dict(n_tiles=1 << 30, heads=4), dict(lse=None), dict(tiles=None)]
+     + [{f: t} for f in "qkvo" for t in BAD_TENSORS]),
+    ("taco_attention_backward", attention_args, [dict(delta=None)] + [{f: t} for f in ("d_o", "d_q", "d_k", "d_v") for t in BAD_TENSORS]),
+    ("taco_attention_step", step_args, [dict(rows=-1), dict(num_pages=0), dict(page_size=0), dict(table_width=0), dict(table=None), dict(lengths=None), dict(k_pages=None),
+                                        dict(v_pages=(1 << 20) + 4), dict(k_page_stride=1022), dict(v_token_stride=-64), dict(scale=-1.0), dict(rows=1 << 30, heads=2),
+                                        dict(k_new=tensor(p=None)), dict(v_new=tensor(p=None)), dict(q=tensor(hs=16))] + [{f: t} for f in ("q", "o") for t in BAD_TENSORS]),
+    ("taco_linear_attention", linear_args, [dict(n_segments=1), dict(n_sequences=-1), dict(scale=0.0), dict(scale=float("inf")), dict(log_decay=None), dict(segments=None),
+                                            dict(first_segment=None), dict(n_segments=90000, n_sequences=80000)] + [{f: t} for f in "qkvo" for t in BAD_TENSORS]),
+    ("taco_linear_attention_backward", linear_args, [{f: t} for f in ("q", "d_o", "d_q", "d_k", "d_v") for t in BAD_TENSORS]),
+    ("taco_linear_attention_step", linear_step_args, [dict(rows=-1), dict(scale=0.0), dict(state=None), dict(state=(1 << 20) + 4), dict(log_decay=None),
+                                                      dict(reset=1 << 20, reset_bytes=2), dict(dim=10)] + [{f: t} for f in "qkvo" for t in BAD_TENSORS])])
+def test_entry_points_refuse(lib, name, make, bad):
+    """before any HIP call, with a message"""
+    f = getattr(lib, name)
+    assert f(None, None) == -1
+    for kw in bad:
+        assert f(C.byref(make(**kw)), None) == -1, kw
+        assert lib.taco_sequence_last_error(), kw
+
+
+def test_workspaces(lib):
+    a = step_args(table_width=4096)
+    need = lib.taco_attention_step_workspace_bytes(C.byref(a))
+    assert need > 0 and lib.taco_attention_step(C.byref(a), None) == -3 and b"workspace" in lib.taco_sequence_last_error()
+    a = step_args(table_width=4096, workspace=1 << 20, workspace_bytes=need - 1)
+    assert lib.taco_attention_step(C.byref(a), None) == -3
+    assert lib.taco_attention_step_workspace_bytes(C.byref(step_args())) == 0
+    a = linear_args(n_segments=5)
+    one, three = (lib.taco_linear_attention_workspace_bytes(C.byref(a), b) for b in (0, 1))
+    assert one == 5 * 2 * 32 * 32 * 4 and three == 3 * one
+    assert lib.taco_linear_attention(C.byref(a), None) == -3 and lib.taco_linear_attention_backward(C.byref(a), None) == -3
+    # nothing to do is not an error, and launches nothing
+    assert lib.taco_attention(C.byref(attention_args(n_tiles=0)), None) == 0
+    assert lib.taco_attention_step(C.byref(step_args(rows=0)), None) == 0
+    assert lib.taco_linear_attention(C.byref(linear_args(n_segments=0, n_sequences=0)), None) == 0
+    assert lib.taco_linear_attention_step(C.byref(linear_step_args(rows=0)), None) == 0
+
+
+def test_host_layer_refuses():
+    z = torch.zeros(4, 2, 32)
+    seqs = sequence.Packed([4], "cuda:0")
+    with pytest.raises(_lib.TacoError, match="MI355X"):
+        sequence.attention(z, z, z, seqs)
+    with pytest.raises(_lib.TacoError, match="MI355X"):
+        sequence.attention_step(z, z, z, z[None], z[None], torch.zeros(4, 1, dtype=torch.int32), torch.zeros(4, dtype=torch.int32))
+    with pytest.raises(_lib.TacoError, match="MI355X"):
+        sequence.linear_attention(z, z, z, torch.zeros(2), seqs)
+    with pytest.raises(_lib.TacoError, match="MI355X"):
+        sequence.linear_attention_step(z, z, z, torch.zeros(2), torch.zeros(4, 2, 32, 32))
+    with pytest.raises(_lib.TacoError, match="MI355X"):
+        sequence.Packed([4], "cpu")
+    for lens in ([-1], [1.5], [[1, 2]], [2 ** 31]):
+        with pytest.raises(ValueError):
+            sequence.Packed(lens, "cuda:0")
+
+
+class Fake:
+    """what the checks look at of a tensor on a HIP device (no such device here)"""
+
+    def __init__(self, shape, dtype=torch.float32, device="cuda:0", grad=False):
+        self.t = torch.empty(shape, dtype=dtype, device="meta")
+        self.device, self.dtype, self.shape, self.requires_grad = torch.device(device), dtype, self.t.shape, grad
+
+    def dim(self):
+        return self.t.dim()
+
+    def __getattr__(self, name):
+        return getattr(self.t, name)
+
+    def data_ptr(self):
+        return 1 << 20
+
+
+def test_host_layer_refuses_shapes_and_types():
+    F, s = Fake, sequence
+    seqs = s.Packed([3, 1], "cuda:0")
+    q, k = F((4, 4, 32)), F((4, 2, 32))
+    for args in [(F((4, 32)), k, k), (q, F((5, 2, 32)), F((5, 2, 32))), (q, F((4, 3, 32)), F((4, 3, 32))), (q, k, F((4, 1, 32))), (q, F((4, 2, 40)), F((4, 2, 40))),
+                 (q, F((4, 2, 32), torch.float16), k), (F((3, 4, 32)), F((3, 2, 32)), F((3, 2, 32))), (F((4, 4, 32), device="cuda:1"), F((4, 2, 32), device="cuda:1"), F((4, 2, 32), device="cuda:1"))]:
+        with pytest.raises(ValueError):
+            s.attention(*args, seqs)
+    with pytest.raises(ValueError):
+        s.attention(q, k, k, [3, 1])
+    for scale in (0, -1.0, float("nan"), float("inf")):
+        with pytest.raises(ValueError):
+            s.attention(q, k, k, seqs, scale=scale)
+    with pytest.raises(ValueError, match="out="):
+        s.attention(F((4, 4, 32), grad=True), k, k, seqs, out=q)
+    for d in (4, 12, 136):
+        with pytest.raises(_lib.TacoError, match="head dimension"):
+            s.attention(*[F((4, 2, d))] * 3, seqs)
+    with pytest.raises(_lib.TacoError, match="float64"):
+        s.attention(*[F((4, 2, 32), torch.float64)] * 3, seqs)
+
+    pages, table, lens = F((6, 16, 2, 32)), F((4, 3), torch.int32), F((4,), torch.int32)
+    for args in [(q, k, None, pages, pages, table, lens), (q, F((3, 2, 32)), k, pages, pages, table, lens), (q, k, k, F((6, 16, 2, 40)), pages, table, lens),
+                 (q, k, k, pages, F((5, 16, 2, 32)), table, lens), (q, k, k, pages, pages, F((4, 3), torch.int64), lens), (q, k, k, pages, pages, table, F((3,), torch.int32)),
+                 (q, k, k, F((6, 16, 2, 32), torch.float16), pages, table, lens), (q, F((4, 3, 32)), F((4, 3, 32)), F((6, 16, 3, 32)), F((6, 16, 3, 32)), table, lens),
+                 (q, k, k, pages, pages, F((4, 0), torch.int32), lens), (q, k, k, F((0, 16, 2, 32)), F((0, 16, 2, 32)), table, lens)]:
+        with pytest.raises(ValueError):
+            s.attention_step(*args)
+    with pytest.raises(_lib.TacoError, match="no gradient"):
+        s.attention_step(F((4, 4, 32), grad=True), k, k, pages, pages, table, lens)
+
+    x, decay = F((4, 2, 32)), F((2,))
+    with pytest.raises(ValueError):
+        s.linear_attention(q, k, k, decay, seqs)
+    with pytest.raises(ValueError):
+        s.linear_attention(x, x, x, F((3,)), seqs)
+    with pytest.raises(_lib.TacoError, match="log_decay"):
+        s.linear_attention(x, x, x, F((2,), grad=True), seqs)
+    with pytest.raises(ValueError):
+        s.linear_attention(x, x, x, decay, seqs, state=F((1, 2, 32, 32)))
+    with pytest.raises(ValueError):
+        s.linear_attention(x, x, x, decay, seqs, scale=0.0)
+    for state, reset in ((F((4, 2, 32, 16)), None), (F((4, 2, 32, 32), torch.float16), None), (F((4, 2, 32, 32)), F((4,), torch.float32)), (F((4, 2, 32, 32)), F((3,), torch.bool))):
+        with pytest.raises(ValueError):
+            s.linear_attention_step(x, x, x, decay, state, reset=reset)
+    with pytest.raises(_lib.TacoError, match="no gradient"):
+        s.linear_attention_step(x, x, x, decay, F((4, 2, 32, 32), grad=True))
+
+
+def lists(monkeypatch, lens):
+    seqs = sequence.Packed(lens, "cuda:0")
+    monkeypatch.setattr(seqs, "_kept", lambda key, make: list(make()) + [None])
+    return seqs
+
+
+@pytest.mark.parametrize("heads", [1, 4, 200])
+@pytest.mark.parametrize("lens", [[1], [0, 5, 0], [64, 65, 128, 129], [1000, 3, 33, 40000], [32] * 500])
+def test_tiles_cover_every_token_once(monkeypatch, lens, heads):
+    seqs = lists(monkeypatch, lens)
+    seen = np.zeros(sum(lens), int)
+    for rows, tiles, key_tiles, count in seqs._tiles(heads):
+        assert rows in (32, 128) and tiles.shape == (count, 4) and tiles.dtype == np.int32
+        assert sorted(map(tuple, tiles)) == sorted(map(tuple, key_tiles))
+        for start, length, first, _ in tiles:
+            assert first % rows == 0 and 0 <= first < length and (start, length) in set(zip(seqs.starts, seqs.lengths))
+            seen[start + first:start + min(first + rows, length)] += 1
+        last = np.minimum(tiles[:, 2] + rows, tiles[:, 1])
+        assert (np.diff(last) <= 0).all()                       # the longest first
+        assert (np.diff(key_tiles[:, 1] - key_tiles[:, 2]) <= 0).all()
+    assert (seen == 1).all()
+
+
+@pytest.mark.parametrize("work", [1, 24, 5000])
+@pytest.mark.parametrize("lens", [[1], [0], [256, 257, 0, 512, 513], [100000, 3], [10] * 2000 + [50000]])
+def test_segments_cover_every_token_once(monkeypatch, lens, work):
+    seqs = lists(monkeypatch, lens)
+    table, first, count = seqs._segments(work)
+    assert table.shape == (count, 8) and first[0] == 0 and first[-1] == count
+    for i, n in enumerate(lens):
+        mine = table[first[i]:first[i + 1]]
+        assert len(mine) >= 1 and (mine[:, 0] == i).all() and (mine[:, 1] == seqs.starts[i]).all() and (mine[:, 2] == n).all()
+        assert (mine[:, 3] == np.cumsum(mine[:, 4]) - mine[:, 4]).all() and mine[:, 4].sum() == n
+        assert (mine[:, 4] > 0).all() or n == 0
+        assert len(mine) == 1 or (mine[:-1, 4] % 64 == 0).all()
+
+
+def test_page_arithmetic_on_the_host(tmp_path):
+    """seq_pages.hpp, the kernel's own functions, compiled with g++ under the address sanitizer: every lookup stays inside its table and names a slot inside the cache, whatever
+    the table and the lengths hold"""
+    src = tmp_path / "t.cpp"
+    src.write_text(r'''
+#include <cassert>
+#include <climits>
+#include <cstdio>
+#include <random>
+#include <vector>
+#include "seq_pages.hpp"
+using namespace seq;
+int main() {
+    std::mt19937 r(1);
+    auto pick = [&](int lo, int hi) { return (int)(lo + r() % (unsigned)(hi - lo + 1)); };
+    assert(keys_of(-1, 4, 16, false) == -1 && keys_of(-1, 4, 16, true) == -1 && keys_of(INT_MIN, 4, 16, true) == -1);
+    assert(keys_of(64, 4, 16, false) == 64 && keys_of(64, 4, 16, true) == -1 && keys_of(63, 4, 16, true) == 64 && keys_of(65, 4, 16, false) == -1);
+    assert(keys_of(0, 1, 1, false) == 0 && keys_of(0, 1, 1, true) == 1);
+    assert(keys_of(INT_MAX, INT_MAX, INT_MAX, true) == -1 && keys_of(INT_MAX, INT_MAX, INT_MAX, false) == -1);      // (room beyond 32 bits)
+    assert(keys_of(1 << 30, 1 << 20, 1 << 20, true) == (1 << 30) + 1);
+    assert(pieces_of(0, 256) == 1 && pieces_of(-1, 256) == 1 && pieces_of(1, 256) == 1 && pieces_of(256, 256) == 1 && pieces_of(257, 256) == 2);
+    for (int n = 0; n < 20000; ++n) {
+        const int width = pick(1, 6), page = pick(1, 40), pages = pick(1, 9);
+        std::vector<int32_t> table(width);
+        const int odd[] = {-1, INT_MIN, INT_MAX, pages, pages + 1};
+        for (auto &e : table) e = pick(0, 9) < 2 ? odd[pick(0, 4)] : pick(0, pages - 1);
+        const int length = pick(-3, width * page + 3);
+        const bool joins = pick(0, 1);
+        const int keys = keys_of(length, width, page, joins);
+        assert(keys == -1 || (keys >= 0 && keys <= width * page && keys == length + (joins ? 1 : 0)));
+        for (int t = 0; t < keys; ++t) {
+            const Place at = place_of(table.data(), t, page, pages);
+            assert(at.page >= 0 && at.page < pages && at.slot >= 0 && at.slot < page);
+            assert(at.bad == (table[t / page] < 0 || table[t / page] >= pages));
+            if (!at.bad) assert(at.page == table[t / page] && at.slot == t % page);
+        }
+    }
+    assert(element_of(Place{1 << 20, 63, false}, (int64_t)1 << 14, 256) == ((int64_t)1 << 34) + 63 * 256);
+    puts("ok");
+}
+''')
+    exe = str(tmp_path / "t")
+    subprocess.check_call(["g++", "-std=c++17", "-O1", "-g", "-fsanitize=address,undefined", "-I", os.path.join(ROOT, "taco_amd", "csrc"), "-o", exe, str(src)])
+    assert subprocess.check_output([exe]).strip() == b"ok"
