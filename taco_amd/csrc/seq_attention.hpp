@@ -28,21 +28,44 @@ __device__ __forceinline__ void locate(int block, int heads, int &tile, int &hea
 
 template <typename T> constexpr int waves_per_simd(int nw) { return nw == 4 && sizeof(T) == 2 ? 2 : 1; }
 
+// acc += X w for a product whose tile X of 32 rows is read by columns: one step of a running sum in acc.  float32 sums each tile apart first: the sum over a long
+// sequence then has a rounding per tile in it, not per pair of rows (its error is the float32 result's own; the 16-bit types' roundings are larger).
+template <typename T, int DP> __device__ __forceinline__ void add_columns(const char *lds, int row0, const f32x16 &w, f32x16 (&acc)[DP / 32], int lane) {
+    frag<T> f[2];
+#pragma unroll
+    for (int x = 0; x < 2; ++x) f[x] = to_frag<T>(w, x);
+    if constexpr (sizeof(T) == 4) {
+#pragma unroll
+        for (int b = 0; b < DP / 32; ++b) {
+            f32x16 y[1];
+            clear(y);
+#pragma unroll
+            for (int x = 0; x < 2; ++x) y[0] = mma(Tile<T, DP>::cols(lds, row0 + 16 * x, 32 * b, lane), f[x], y[0]);
+            acc[b] += y[0];
+        }
+    } else {
+#pragma unroll
+        for (int x = 0; x < 2; ++x)
+#pragma unroll
+            for (int b = 0; b < DP / 32; ++b) acc[b] = mma(Tile<T, DP>::cols(lds, row0 + 16 * x, 32 * b, lane), f[x], acc[b]);
+    }
+}
+
 // Forward.  A wavefront owns 32 queries (columns of all its products), a workgroup NW of them and one K and one V tile of BN keys in LDS; the next tiles travel
 // in registers meanwhile.  S^T = K Q^T leaves a query's scores in one lane and its other half: the softmax needs one exchange per tile, and P^T is the next
 // product's operand as it stands (O^T = V^T P^T).  P is rounded to the inputs' type for that product (half a step, independent from key to key, so about
 // as much as the output's own rounding); its sum stays float32.
-// Keys run from the diagonal to the first one: the only tile with hidden keys of the sequence comes first, while O is zero, so if a hidden NaN got into O
-// it shows there and the tile is done again without it.
+// Keys run from the diagonal to the first one.  The tiles that hide keys come first, in a loop of their own, and the others run without a mask.
 template <typename T, int DP, int NW>
 __global__ __launch_bounds__(64 * NW, waves_per_simd<T>(NW)) void attention_kernel(AttentionParams p) {
     typedef Tile<T, DP> tile;
     constexpr int BM = 32 * NW, BN = NW == 1 ? 32 : 64, NB = BN / 32, NS = DP / 16, DB = DP / 32, NT = 64 * NW;
     __shared__ __attribute__((aligned(16))) char lds_k[BN * tile::ROW], lds_v[BN * tile::ROW];
+    __shared__ int nonfinite;
     int ti, head;
     locate(blockIdx.x, p.heads, ti, head);
     const taco_seq_tile w = p.tiles[ti];
-    const int kvh = head / (p.heads / p.kv_heads), t = threadIdx.x, lane = t & 63, wave = t >> 6, h = lane >> 5, d = p.dim;
+    const int kvh = head / (p.heads / p.kv_heads), t = threadIdx.x, lane = t & 63, wave = __builtin_amdgcn_readfirstlane(t >> 6), h = lane >> 5, d = p.dim;
     const int first = w.first + 32 * wave, row = first + (lane & 31);
     const uint32_t rb = d * sizeof(T);
     const float c = p.scale * LOG2E;
@@ -66,29 +89,14 @@ __global__ __launch_bounds__(64 * NW, waves_per_simd<T>(NW)) void attention_kern
     float m = -__builtin_inff(), l = 0.f;
     const int last = p.causal ? min(w.length, w.first + BM) - 1 : w.length - 1;
     const int limit = p.causal ? row : w.length - 1;       // the last key this lane's query sees
-    int kt = last / BN;
-    fetch(kt);
-    for (; kt >= 0; --kt) {
-        __syncthreads();
-        sk.put(lds_k, t);
-        sv.put(lds_v, t);
-        __syncthreads();
-        if (kt > 0) fetch(kt - 1);
-        const int k0 = kt * BN;
-        if (p.causal && k0 > first + 31) continue;      // (the wavefront's: all of the tile is hidden)
-        f32x16 s[NB];
+    auto scores = [&](f32x16 (&s)[NB]) {
         clear(s);
 #pragma unroll
         for (int n = 0; n < NB; ++n)
 #pragma unroll
             for (int x = 0; x < NS; ++x) s[n] = mma(tile::rows(lds_k, 32 * n, x, lane), qf[x], s[n]);
-        const bool masked = k0 + BN - 1 > (p.causal ? first : w.length - 1);
-        if (masked) {
-#pragma unroll
-            for (int n = 0; n < NB; ++n)
-#pragma unroll
-                for (int i = 0; i < 16; ++i) s[n][i] = k0 + 32 * n + row_of(i, h) <= limit ? s[n][i] : -__builtin_inff();
-        }
+    };
+    auto softmax = [&](f32x16 (&s)[NB]) {
         float mx = s[0][0];
 #pragma unroll
         for (int n = 0; n < NB; ++n)
@@ -100,32 +108,78 @@ __global__ __launch_bounds__(64 * NW, waves_per_simd<T>(NW)) void attention_kern
             float a = exp2_(m * c - mu);
             l *= a;
 #pragma unroll
-            for (int b = 0; b < DB; ++b)
-#pragma unroll
-                for (int i = 0; i < 16; ++i) o[b][i] *= a;
+            for (int b = 0; b < DB; ++b) o[b] *= a;
             m = mn;
         }
+        float sum[4] = {0.f, 0.f, 0.f, 0.f};
 #pragma unroll
         for (int n = 0; n < NB; ++n)
 #pragma unroll
             for (int i = 0; i < 16; ++i) {
                 s[n][i] = exp2_(s[n][i] * c - mu);
-                l += s[n][i];
+                sum[i % 4] += s[n][i];
             }
+        l += (sum[0] + sum[1]) + (sum[2] + sum[3]);
+    };
+
+    int kt = last / BN;
+    // tiles from here up hide keys of the sequence from some query of the workgroup (causal), or hold rows behind its end
+    const int whole = p.causal ? w.first / BN : w.length / BN;
+    fetch(kt);
+    if (t == 0) nonfinite = 0;
+    for (; kt >= whole; --kt) {
+        __syncthreads();
+        const bool bad = p.causal && __any(sv.any_nonfinite());
+        if (bad) {
+            sv.nonfinite_to_zero();
+            if (lane == 0) nonfinite = kt + 1;
+        }
+        sk.put(lds_k, t);
+        sv.put(lds_v, t);
+        __syncthreads();
+        if (kt > 0) fetch(kt - 1);
+        const int k0 = kt * BN;
+        if (p.causal && k0 > first + 31) continue;      // (the wavefront's: all of the tile is hidden)
+        f32x16 s[NB];
+        scores(s);
 #pragma unroll
         for (int n = 0; n < NB; ++n)
 #pragma unroll
-            for (int x = 0; x < 2; ++x) {
-                frag<T> pf = to_frag<T>(s[n], x);
+            for (int i = 0; i < 16; ++i) s[n][i] = k0 + 32 * n + row_of(i, h) <= limit ? s[n][i] : -__builtin_inff();
+        softmax(s);
 #pragma unroll
-                for (int b = 0; b < DB; ++b) o[b] = mma(tile::cols(lds_v, 32 * n + 16 * x, 32 * b, lane), pf, o[b]);
+        for (int n = 0; n < NB; ++n) add_columns<T, DP>(lds_v, 32 * n, s[n], o, lane);
+        if (nonfinite == kt + 1) {
+            for (int b = 0; b < DP; b += 64) {
+                int plus, minus;
+                const int n = min(BN, w.length - k0);
+                first_nonfinite<T>(vp + (int64_t)k0 * p.v.ts, p.v.ts, b + lane < d ? n : 0, b + lane < d ? b + lane : 0, plus, minus);
+                if (b + lane >= d) plus = minus = n;
+                plus += k0;
+                minus += k0;
+                const int end = k0 + n;
+#pragma unroll
+                for (int x = 0; x < DB; ++x)
+                    if (32 * x >= b && 32 * x < b + 64)
+#pragma unroll
+                        for (int i = 0; i < 16; ++i) {
+                            const int from = 32 * x - b + row_of(i, h), fp = __shfl(plus, from), fm = __shfl(minus, from);
+                            o[x][i] += (fp < end && fp <= limit ? __builtin_inff() : 0.f) + (fm < end && fm <= limit ? -__builtin_inff() : 0.f);
+                        }
             }
-        if (masked && p.causal && any_nan(o)) {
-            clear(o);
-#pragma unroll
-            for (int n = 0; n < NB; ++n)
-                accumulate_seen<T, DP>(lds_v, 32 * n, 0, s[n], [&](int r) { return k0 + 32 * n + r <= limit; }, o, lane);
         }
+    }
+    for (; kt >= 0; --kt) {
+        __syncthreads();
+        sk.put(lds_k, t);
+        sv.put(lds_v, t);
+        __syncthreads();
+        if (kt > 0) fetch(kt - 1);
+        f32x16 s[NB];
+        scores(s);
+        softmax(s);
+#pragma unroll
+        for (int n = 0; n < NB; ++n) add_columns<T, DP>(lds_v, 32 * n, s[n], o, lane);
     }
     l += other_half(l);
     if (row < w.length) {
@@ -137,15 +191,18 @@ __global__ __launch_bounds__(64 * NW, waves_per_simd<T>(NW)) void attention_kern
 // Backward, first launch: dQ, and delta = rowsum(dO O) for the second.  The forward kernel's shape: dS^T = P^T (dP^T - delta) from S^T = K Q^T and
 // dP^T = V dO^T, then dQ^T = K^T dS^T, K read both ways from one LDS tile.  dQ and dK / dV take a kernel each, which computes S and dP twice (seven
 // products for five), because neither then needs an atomic or a float32 copy of a gradient.
+// A query that sees few keys has gradients that are small differences of dP and delta, and o as it was rounded would set their error.  Where all its keys
+// lie in one tile, delta is the sum of P dP over that tile instead, in float32.
 template <typename T, int DP, int NW>
 __global__ __launch_bounds__(64 * NW, 1) void attention_dq_kernel(AttentionParams p) {
     typedef Tile<T, DP> tile;
     constexpr int BM = 32 * NW, BN = NW == 1 ? 32 : 64, NB = BN / 32, NS = DP / 16, DB = DP / 32, NT = 64 * NW;
     __shared__ __attribute__((aligned(16))) char lds_k[BN * tile::ROW], lds_v[BN * tile::ROW];
+    __shared__ int nonfinite;       // the first key of the tile with something not finite in it
     int ti, head;
     locate(blockIdx.x, p.heads, ti, head);
     const taco_seq_tile w = p.tiles[ti];
-    const int kvh = head / (p.heads / p.kv_heads), t = threadIdx.x, lane = t & 63, wave = t >> 6, h = lane >> 5, d = p.dim;
+    const int kvh = head / (p.heads / p.kv_heads), t = threadIdx.x, lane = t & 63, wave = __builtin_amdgcn_readfirstlane(t >> 6), h = lane >> 5, d = p.dim;
     const int first = w.first + 32 * wave, row = first + (lane & 31);
     const uint32_t rb = d * sizeof(T);
     const float c = p.scale * LOG2E;
@@ -167,12 +224,8 @@ __global__ __launch_bounds__(64 * NW, 1) void attention_dq_kernel(AttentionParam
         }
         delta += other_half(delta);
     }
-    float lse = 0.f;
-    if (row < w.length) {
-        const int64_t at = (int64_t)(w.start + row) * p.heads + head;
-        lse = p.lse[at];
-        if (h == 0) p.delta[at] = delta;
-    }
+    const int64_t at = (int64_t)(w.start + row) * p.heads + head;
+    const float lse = row < w.length ? p.lse[at] : 0.f;
     const float mu = lse == -__builtin_inff() ? __builtin_inff() : lse * LOG2E;      // (a row that attends to nothing: P = 0)
     const char *kp = p.k.p + (int64_t)w.start * p.k.ts + kvh * p.k.hs, *vp = p.v.p + (int64_t)w.start * p.v.ts + kvh * p.v.hs;
     Staged<T, DP, BN, NT> sk, sv;
@@ -186,47 +239,93 @@ __global__ __launch_bounds__(64 * NW, 1) void attention_dq_kernel(AttentionParam
     clear(dq);
     const int last = p.causal ? min(w.length, w.first + BM) - 1 : w.length - 1;
     const int limit = p.causal ? row : w.length - 1;
+    // P and P (dP - delta) of 32 keys
+    auto weights = [&](int n, f32x16 &pr, f32x16 &dp) {
+        f32x16 x[2];
+        clear(x);
+#pragma unroll
+        for (int y = 0; y < NS; ++y) x[0] = mma(tile::rows(lds_k, 32 * n, y, lane), qf[y], x[0]);
+#pragma unroll
+        for (int y = 0; y < NS; ++y) x[1] = mma(tile::rows(lds_v, 32 * n, y, lane), gf[y], x[1]);
+#pragma unroll
+        for (int i = 0; i < 16; ++i) pr[i] = exp2_(x[0][i] * c - mu);
+        dp = x[1];
+    };
     int kt = last / BN;
+    const int whole = p.causal ? w.first / BN : w.length / BN;
     fetch(kt);
+    if (t == 0) nonfinite = BN;
+    for (; kt >= whole; --kt) {
+        __syncthreads();
+        if (p.causal && __any(sk.any_nonfinite())) {
+            int r = BN;
+#pragma unroll
+            for (int i = Staged<T, DP, BN, NT>::N - 1; i >= 0; --i)
+                if (sk.chunk_nonfinite(i)) r = (i * NT + t) / tile::NC;
+            sk.nonfinite_to_zero();
+            atomicMin(&nonfinite, r);
+        }
+        sk.put(lds_k, t);
+        sv.put(lds_v, t);
+        __syncthreads();
+        const int seen_bad = nonfinite;
+        if (kt > 0) fetch(kt - 1);
+        const int k0 = kt * BN;
+        if (!(p.causal && k0 > first + 31)) {      // (else: all of the tile is hidden from the wavefront)
+            f32x16 pr[NB], ds[NB];
+#pragma unroll
+            for (int n = 0; n < NB; ++n) {
+                weights(n, pr[n], ds[n]);
+#pragma unroll
+                for (int i = 0; i < 16; ++i) {
+                    const bool seen = k0 + 32 * n + row_of(i, h) <= limit;
+                    pr[n][i] = seen ? pr[n][i] : 0.f;
+                    ds[n][i] = seen ? ds[n][i] : 0.f;
+                }
+            }
+            if (k0 == 0) {
+                float x = 0.f;
+#pragma unroll
+                for (int n = 0; n < NB; ++n)
+#pragma unroll
+                    for (int i = 0; i < 16; ++i) x += pr[n][i] * ds[n][i];
+                delta = limit < BN ? x + other_half(x) : delta;
+            }
+#pragma unroll
+            for (int n = 0; n < NB; ++n) {
+#pragma unroll
+                for (int i = 0; i < 16; ++i) ds[n][i] = k0 + 32 * n + row_of(i, h) <= limit ? pr[n][i] * (ds[n][i] - delta) : 0.f;
+                add_columns<T, DP>(lds_k, 32 * n, ds[n], dq, lane);
+            }
+            if (k0 + seen_bad <= limit && seen_bad < BN) {      // (a key that is not finite: its weight is not either)
+#pragma unroll
+                for (int b = 0; b < DB; ++b) dq[b] += __builtin_nanf("");
+            }
+        }
+        if (p.causal) {
+            __syncthreads();
+            if (t == 0) nonfinite = BN;
+        }
+    }
     for (; kt >= 0; --kt) {
         __syncthreads();
         sk.put(lds_k, t);
         sv.put(lds_v, t);
         __syncthreads();
         if (kt > 0) fetch(kt - 1);
-        const int k0 = kt * BN;
-        if (p.causal && k0 > first + 31) continue;
-        const bool masked = k0 + BN - 1 > (p.causal ? first : w.length - 1);
-        f32x16 ds[NB];
 #pragma unroll
         for (int n = 0; n < NB; ++n) {
-            f32x16 x[2];
-            clear(x);
+            f32x16 pr, ds;
+            weights(n, pr, ds);
 #pragma unroll
-            for (int y = 0; y < NS; ++y) x[0] = mma(tile::rows(lds_k, 32 * n, y, lane), qf[y], x[0]);
-#pragma unroll
-            for (int y = 0; y < NS; ++y) x[1] = mma(tile::rows(lds_v, 32 * n, y, lane), gf[y], x[1]);
-#pragma unroll
-            for (int i = 0; i < 16; ++i) ds[n][i] = exp2_(x[0][i] * c - mu) * (x[1][i] - delta);
-            if (masked) {
-#pragma unroll
-                for (int i = 0; i < 16; ++i) ds[n][i] = k0 + 32 * n + row_of(i, h) <= limit ? ds[n][i] : 0.f;
-            }
-#pragma unroll
-            for (int y = 0; y < 2; ++y) {
-                frag<T> f = to_frag<T>(ds[n], y);
-#pragma unroll
-                for (int b = 0; b < DB; ++b) dq[b] = mma(tile::cols(lds_k, 32 * n + 16 * y, 32 * b, lane), f, dq[b]);
-            }
-        }
-        if (masked && p.causal && any_nan(dq)) {
-            clear(dq);
-#pragma unroll
-            for (int n = 0; n < NB; ++n)
-                accumulate_seen<T, DP>(lds_k, 32 * n, 0, ds[n], [&](int r) { return k0 + 32 * n + r <= limit; }, dq, lane);
+            for (int i = 0; i < 16; ++i) ds[i] = pr[i] * (ds[i] - delta);
+            add_columns<T, DP>(lds_k, 32 * n, ds, dq, lane);
         }
     }
-    if (row < w.length) store_row<T>((T *)(p.d_q.p + (int64_t)(w.start + row) * p.d_q.ts + head * p.d_q.hs), dq, p.scale, d, lane);
+    if (row < w.length) {
+        store_row<T>((T *)(p.d_q.p + (int64_t)(w.start + row) * p.d_q.ts + head * p.d_q.hs), dq, p.scale, d, lane);
+        if (h == 0) p.delta[at] = delta;
+    }
 }
 
 // Backward, second launch: dK and dV.  A wavefront owns 32 keys, whose K and V rows stay in registers as operands; Q and dO tiles of BQ queries pass through LDS,
@@ -238,10 +337,11 @@ __global__ __launch_bounds__(64 * NW, 1) void attention_dkv_kernel(AttentionPara
     constexpr int BK = 32 * NW, BQ = NW == 1 ? 32 : 64, NB = BQ / 32, NS = DP / 16, DB = DP / 32, NT = 64 * NW;
     __shared__ __attribute__((aligned(16))) char lds_q[BQ * tile::ROW], lds_g[BQ * tile::ROW];
     __shared__ __attribute__((aligned(16))) float lds_mu[BQ], lds_delta[BQ];
+    __shared__ int nonfinite;       // the last query of the tile with something not finite in its row or its gradient's
     int ti, kvh;
     locate(blockIdx.x, p.kv_heads, ti, kvh);
     const taco_seq_tile w = p.key_tiles[ti];
-    const int t = threadIdx.x, lane = t & 63, wave = t >> 6, h = lane >> 5, d = p.dim, G = p.heads / p.kv_heads;
+    const int t = threadIdx.x, lane = t & 63, wave = __builtin_amdgcn_readfirstlane(t >> 6), h = lane >> 5, d = p.dim, G = p.heads / p.kv_heads;
     const int first = w.first + 32 * wave, key = first + (lane & 31);
     const uint32_t rb = d * sizeof(T);
     const float c = p.scale * LOG2E;
@@ -257,11 +357,12 @@ __global__ __launch_bounds__(64 * NW, 1) void attention_dkv_kernel(AttentionPara
             vf[s] = rows_global<T>(rv, p.v.ts, d, 32 * wave, s, lane);
         }
     }
-    const int qt0 = p.causal ? w.first / BQ : 0, nq = (w.length - 1) / BQ + 1 - qt0;
+    const int qt0 = p.causal ? w.first / BQ : 0, qt1 = (w.length - 1) / BQ + 1;
+    const int whole = p.causal ? min(qt1, (w.first + BK) / BQ) : 0;      // tiles from here on hide no key of the workgroup
     Staged<T, DP, BQ, NT> sq, sg;
     float mu_r = 0.f, delta_r = 0.f;
-    auto fetch = [&](int it) {
-        const int head = kvh * G + it / nq, q0 = (qt0 + it % nq) * BQ, n = min(BQ, w.length - q0);
+    auto fetch = [&](int head, int qt) {
+        const int q0 = qt * BQ, n = min(BQ, w.length - q0);
         const int64_t at = w.start + q0;
         sq.load(rows_of(p.q.p + at * p.q.ts + head * p.q.hs, n, p.q.ts, rb), p.q.ts, d, t);
         sg.load(rows_of(p.d_o.p + at * p.d_o.ts + head * p.d_o.hs, n, p.d_o.ts, rb), p.d_o.ts, d, t);
@@ -271,65 +372,94 @@ __global__ __launch_bounds__(64 * NW, 1) void attention_dkv_kernel(AttentionPara
             mu_r = lse == -__builtin_inff() ? __builtin_inff() : lse * LOG2E;
         }
     };
-
-    f32x16 dk[DB], dv[DB];
-    clear(dk);
-    clear(dv);
-    fetch(0);
-    for (int it = 0; it < G * nq; ++it) {
-        __syncthreads();
+    auto put = [&]() {
         sq.put(lds_q, t);
         sg.put(lds_g, t);
         if (t < BQ) {
             lds_mu[t] = mu_r;
             lds_delta[t] = delta_r;
         }
-        __syncthreads();
-        if (it + 1 < G * nq) fetch(it + 1);
-        const int q0 = (qt0 + it % nq) * BQ;
+    };
+
+    f32x16 dk[DB], dv[DB];
+    clear(dk);
+    clear(dv);
+    // P and dS of 32 queries
+    auto weights = [&](int n, f32x16 (&x)[2]) {
+        clear(x);
 #pragma unroll
-        for (int n = 0; n < NB; ++n) {
-            const int qb = q0 + 32 * n;
-            if (p.causal && qb < first) continue;       // (all of the block comes before the wavefront's keys)
-            f32x16 x[2];
-            clear(x);
+        for (int y = 0; y < NS; ++y) x[0] = mma(tile::rows(lds_q, 32 * n, y, lane), kf[y], x[0]);
 #pragma unroll
-            for (int y = 0; y < NS; ++y) x[0] = mma(tile::rows(lds_q, 32 * n, y, lane), kf[y], x[0]);
+        for (int y = 0; y < NS; ++y) x[1] = mma(tile::rows(lds_g, 32 * n, y, lane), vf[y], x[1]);
 #pragma unroll
-            for (int y = 0; y < NS; ++y) x[1] = mma(tile::rows(lds_g, 32 * n, y, lane), vf[y], x[1]);
+        for (int i = 0; i < 16; i += 4) {
+            f32x4 mu = *(const f32x4 *)(lds_mu + 32 * n + row_of(i, h)), de = *(const f32x4 *)(lds_delta + 32 * n + row_of(i, h));
 #pragma unroll
-            for (int i = 0; i < 16; i += 4) {
-                f32x4 mu = *(const f32x4 *)(lds_mu + 32 * n + row_of(i, h)), de = *(const f32x4 *)(lds_delta + 32 * n + row_of(i, h));
-#pragma unroll
-                for (int j = 0; j < 4; ++j) {
-                    x[0][i + j] = exp2_(x[0][i + j] * c - mu[j]);
-                    x[1][i + j] = x[0][i + j] * (x[1][i + j] - de[j]);
-                }
+            for (int j = 0; j < 4; ++j) {
+                x[0][i + j] = exp2_(x[0][i + j] * c - mu[j]);
+                x[1][i + j] = x[0][i + j] * (x[1][i + j] - de[j]);
             }
-            const bool masked = p.causal && qb == first;
-            bool apart = false;
-            if (masked) {
+        }
+    };
+    fetch(kvh * G, qt0);
+    if (t == 0) nonfinite = -1;
+    for (int head = kvh * G; head < (kvh + 1) * G; ++head) {
+        int qt = qt0;
+        auto next = [&]() {
+            if (qt + 1 < qt1) fetch(head, qt + 1);
+            else if (head + 1 < (kvh + 1) * G) fetch(head + 1, qt0);
+        };
+        for (; qt < whole; ++qt) {
+            __syncthreads();
+            if (__any(sq.any_nonfinite() || sg.any_nonfinite())) {
+                int r = -1;
+#pragma unroll
+                for (int i = 0; i < Staged<T, DP, BQ, NT>::N; ++i)
+                    if (sq.chunk_nonfinite(i) || sg.chunk_nonfinite(i)) r = (i * NT + t) / tile::NC;
+                sq.nonfinite_to_zero();
+                sg.nonfinite_to_zero();
+                atomicMax(&nonfinite, r);
+            }
+            put();
+            __syncthreads();
+            const int seen_bad = nonfinite;
+            next();
+#pragma unroll
+            for (int n = 0; n < NB; ++n) {
+                const int qb = qt * BQ + 32 * n;
+                if (qb < first) continue;       // (all of the block comes before the wavefront's keys)
+                f32x16 x[2];
+                weights(n, x);
 #pragma unroll
                 for (int i = 0; i < 16; ++i) {
-                    bool seen = key <= qb + row_of(i, h);
+                    const bool seen = key <= qb + row_of(i, h);
                     x[0][i] = seen ? x[0][i] : 0.f;
                     x[1][i] = seen ? x[1][i] : 0.f;
                 }
-                apart = tile::any_nonfinite(lds_q, 32 * n, 32, lane) || tile::any_nonfinite(lds_g, 32 * n, 32, lane);
+                add_columns<T, DP>(lds_g, 32 * n, x[0], dv, lane);
+                add_columns<T, DP>(lds_q, 32 * n, x[1], dk, lane);
             }
-            if (apart) {
-                auto seen = [&](int r) { return key <= qb + r; };
-                accumulate_seen<T, DP>(lds_g, 32 * n, 0, x[0], seen, dv, lane);
-                accumulate_seen<T, DP>(lds_q, 32 * n, 0, x[1], seen, dk, lane);
-            } else {
+            if (seen_bad >= 0 && key <= qt * BQ + seen_bad) {       // (a key that such a query sees: its gradients are not finite)
 #pragma unroll
-                for (int y = 0; y < 2; ++y) {
-                    frag<T> pf = to_frag<T>(x[0], y), sf = to_frag<T>(x[1], y);
-#pragma unroll
-                    for (int b = 0; b < DB; ++b) dv[b] = mma(tile::cols(lds_g, 32 * n + 16 * y, 32 * b, lane), pf, dv[b]);
-#pragma unroll
-                    for (int b = 0; b < DB; ++b) dk[b] = mma(tile::cols(lds_q, 32 * n + 16 * y, 32 * b, lane), sf, dk[b]);
+                for (int b = 0; b < DB; ++b) {
+                    dk[b] += __builtin_nanf("");
+                    dv[b] += __builtin_nanf("");
                 }
+            }
+            __syncthreads();
+            if (t == 0) nonfinite = -1;
+        }
+        for (; qt < qt1; ++qt) {
+            __syncthreads();
+            put();
+            __syncthreads();
+            next();
+#pragma unroll
+            for (int n = 0; n < NB; ++n) {
+                f32x16 x[2];
+                weights(n, x);
+                add_columns<T, DP>(lds_g, 32 * n, x[0], dv, lane);
+                add_columns<T, DP>(lds_q, 32 * n, x[1], dk, lane);
             }
         }
     }

@@ -114,22 +114,6 @@ template <typename T, int DP> struct Tile {
             return f;
         }
     }
-    // does any element of rows [row0, row0 + n) differ from a finite number?  (wave-uniform answer; every lane takes chunks in turn)
-    static __device__ __forceinline__ bool any_nonfinite(const char *lds, int row0, int n, int lane) {
-        bool bad = false;
-        for (int e = lane; e < n * NC; e += 64) {
-            u32x4 x = *(const u32x4 *)(lds + at(row0 + e / NC, e % NC));
-#pragma unroll
-            for (int i = 0; i < 4; ++i) {
-                if constexpr (sizeof(T) == 4) bad |= (x[i] & 0x7f800000u) == 0x7f800000u;
-                else {
-                    constexpr uint32_t m = __is_same(T, f16) ? 0x7c00u : 0x7f80u;
-                    bad |= (x[i] & m) == m || (x[i] & (m << 16)) == (m << 16);
-                }
-            }
-        }
-        return __any(bad);
-    }
 };
 
 // ---- Global memory.  A buffer descriptor covers the rows of one tile that exist; what lies outside reads as zero, so no lane branches and padding rows and
@@ -170,6 +154,30 @@ template <typename T, int DP, int ROWS, int NT> struct Staged {
             tile::put(lds, e / tile::NC, e % tile::NC, x[i]);
         }
     }
+    // NaN and infinities have an exponent of all ones: adding one to its last place carries into the sign's bit, which is masked out first
+    static constexpr uint32_t MAGNITUDE = sizeof(T) == 4 ? 0x7fffffffu : 0x7fff7fffu, SIGNS = ~MAGNITUDE,
+                              STEP = sizeof(T) == 4 ? 0x00800000u : __is_same(T, f16) ? 0x04000400u : 0x00800080u;
+    __device__ __forceinline__ bool any_nonfinite() const {
+        bool bad = false;
+#pragma unroll
+        for (int i = 0; i < N; ++i) bad |= chunk_nonfinite(i);
+        return bad;
+    }
+    __device__ __forceinline__ bool chunk_nonfinite(int i) const {
+        uint32_t bad = 0;
+#pragma unroll
+        for (int j = 0; j < 4; ++j) bad |= (x[i][j] & MAGNITUDE) + STEP;
+        return bad & SIGNS;
+    }
+    __device__ __forceinline__ void nonfinite_to_zero() {
+#pragma unroll
+        for (int i = 0; i < N; ++i)
+#pragma unroll
+            for (int j = 0; j < 4; ++j) {
+                uint32_t bad = ((x[i][j] & MAGNITUDE) + STEP) & SIGNS;      // the sign bits of what goes
+                x[i][j] &= sizeof(T) == 4 ? (bad ? 0u : ~0u) : ~((bad >> 15) * 0xffffu);
+            }
+    }
 };
 
 // operand whose lane is a row of global memory (row0 + l % 32), contraction over the columns 16 s + 8 h + j
@@ -205,54 +213,19 @@ template <typename T, int DB> __device__ __forceinline__ void store_row(T *row, 
         }
 }
 
-// acc[dim][lane's column] += sum over the 32 rows from row0 of X[row][dim] * w[row][column], where rows that are hidden from a column hold NaN or infinities:
-// their w is 0, but a plain matrix product makes NaN of 0 * NaN.  The finite part goes through the product as it is.  What is not finite is counted over
-// the rows a column sees, apart for each sign of the term (a NaN, or a weight of 0, counts for both), and joins as +inf, -inf or their sum, NaN.
-// Runs only where something not finite turned up.
-template <typename T> __device__ __forceinline__ frag<T> part_of(frag<T> f, int which) {      // 0: what is finite; 1: marks of +inf and NaN; 2: of -inf and NaN
-#pragma unroll
-    for (int j = 0; j < 8; ++j) {
-        float x = (float)f[j];
-        bool fin = __builtin_fabsf(x) < __builtin_inff();
-        f[j] = which == 0 ? (fin ? f[j] : (T)0.f) : (T)(!fin && !(which == 1 ? x < 0.f : x > 0.f) ? 1.f : 0.f);
+// ---- Hidden rows that are not finite.  A tile in which rows of a sequence are hidden from some columns goes through a matrix product with weights of 0 for
+// them, and 0 * NaN is NaN.  Such a tile (only those on the diagonal) is therefore looked over on its way into LDS, three operations for four bytes; if
+// anything in it is not finite, it is written without that, a flag says so, and the few lines below put what the columns do see back in: rare, and slow.
+
+// Column `col` of n rows of global memory: the first row that holds +inf or NaN, and the first that holds -inf or NaN (n: none)
+template <typename T> __device__ inline void first_nonfinite(const char *base, int64_t stride_bytes, int n, int col, int &plus, int &minus) {
+    plus = minus = n;
+    for (int r = n - 1; r >= 0; --r) {
+        const float x = (float)((const T *)(base + r * stride_bytes))[col];
+        if (__builtin_fabsf(x) < __builtin_inff()) continue;
+        if (!(x < 0.f)) plus = r;
+        if (!(x > 0.f)) minus = r;
     }
-    return f;
-}
-template <typename T, int DP, int NB, typename F>
-__device__ __forceinline__ void accumulate_seen(const char *lds, int row0, int col0, const f32x16 &w, F seen, f32x16 (&acc)[NB], int lane) {
-    frag<T> f[2], up[2], down[2];
-#pragma unroll
-    for (int s = 0; s < 2; ++s) {
-        f[s] = to_frag<T>(w, s);
-#pragma unroll
-        for (int j = 0; j < 8; ++j) {
-            bool v = seen(row_of(8 * s + j, lane >> 5));
-            up[s][j] = (T)(v && (float)f[s][j] >= 0.f ? 1.f : 0.f);
-            down[s][j] = (T)(v && (float)f[s][j] <= 0.f ? 1.f : 0.f);
-        }
-    }
-#pragma unroll
-    for (int b = 0; b < NB; ++b) {
-        f32x16 n[2];
-        clear(n);
-#pragma unroll
-        for (int s = 0; s < 2; ++s) {
-            frag<T> x = Tile<T, DP>::cols(lds, row0 + 16 * s, col0 + 32 * b, lane), p = part_of<T>(x, 1), m = part_of<T>(x, 2);
-            acc[b] = mma(part_of<T>(x, 0), f[s], acc[b]);
-            n[0] = mma(m, down[s], mma(p, up[s], n[0]));
-            n[1] = mma(m, up[s], mma(p, down[s], n[1]));
-        }
-#pragma unroll
-        for (int i = 0; i < 16; ++i) acc[b][i] += (n[0][i] > 0.f ? __builtin_inff() : 0.f) + (n[1][i] > 0.f ? -__builtin_inff() : 0.f);
-    }
-}
-template <int N> __device__ __forceinline__ bool any_nan(const f32x16 (&x)[N]) {
-    bool bad = false;
-#pragma unroll
-    for (int n = 0; n < N; ++n)
-#pragma unroll
-        for (int i = 0; i < 16; ++i) bad |= x[n][i] != x[n][i];
-    return __any(bad);
 }
 
 }  // namespace seq

@@ -90,8 +90,9 @@ __global__ __launch_bounds__(2 * DP, 1) void linear_kernel(LinearParams p) {
     typedef Tile<T, DP> tile;
     constexpr int C = 64, NT = 2 * DP, NS = DP / 16, DB = DP / 32;
     __shared__ __attribute__((aligned(16))) char lds_k[C * tile::ROW], lds_v[C * tile::ROW], lds_q[STATES ? 16 : C * tile::ROW];
+    __shared__ int nonfinite;        // the chunk (its first token) whose V holds something not finite
     const LinearMode m = p.mode[blockIdx.z];
-    const int head = blockIdx.y, t = threadIdx.x, lane = t & 63, wave = t >> 6, h = lane >> 5, d = p.dim;
+    const int head = blockIdx.y, t = threadIdx.x, lane = t & 63, wave = __builtin_amdgcn_readfirstlane(t >> 6), h = lane >> 5, d = p.dim;
     const taco_seq_segment g = p.segments[blockIdx.x];
     const uint32_t rb = d * sizeof(T);
     const float ld = decay2(p.log_decay, head);
@@ -152,13 +153,26 @@ __global__ __launch_bounds__(2 * DP, 1) void linear_kernel(LinearParams p) {
         }
     };
     if (g.count > 0) fetch(0);
+    if (t == 0) nonfinite = -1;
     for (int c0 = 0; c0 < g.count; c0 += C) {
         const int n = min(C, g.count - c0);
         __syncthreads();
+        if (!STATES && __any(sv.any_nonfinite())) {
+            sv.nonfinite_to_zero();
+            if (lane == 0) nonfinite = c0;
+        }
         sk.put(lds_k, t);
         sv.put(lds_v, t);
         if (!STATES) sq.put(lds_q, t);
         __syncthreads();
+        int bad = C;        // the first token of the chunk whose V is not finite in this lane's column
+        if (!STATES && nonfinite == c0) {
+            const int col = 32 * wave + (lane & 31), f = g.first + c0;
+            const char *v = m.v.p + (g.start + (m.reverse ? g.length - 1 - f : f)) * m.v.ts + head * m.v.hs;
+            int plus, minus;
+            first_nonfinite<T>(v, m.reverse ? -m.v.ts : m.v.ts, col < d ? n : 0, col < d ? col : 0, plus, minus);
+            if (col < d && min(plus, minus) < n) bad = min(plus, minus);
+        }
         if (c0 + C < g.count) fetch(c0 + C);
         if (!STATES) {
 #pragma unroll
@@ -167,7 +181,7 @@ __global__ __launch_bounds__(2 * DP, 1) void linear_kernel(LinearParams p) {
                 f32x16 o[1], x[1], y[1];
                 clear(o);
                 clear(y);
-                // the chunk itself.  The hidden half of the triangle first, while o is zero: a hidden NaN shows there
+                // the chunk itself
 #pragma unroll
                 for (int kb = qb; kb >= 0; --kb) {
                     clear(x);
@@ -177,10 +191,6 @@ __global__ __launch_bounds__(2 * DP, 1) void linear_kernel(LinearParams p) {
                     for (int i = 0; i < 16; ++i) x[0][i] = kb == qb ? ((lane & 31) >= row_of(i, h) ? x[0][i] * w0[i] : 0.f) : x[0][i] * w1[i];
 #pragma unroll
                     for (int e = 0; e < 2; ++e) o[0] = mma(tile::cols(lds_v, 32 * kb + 16 * e, 32 * wave, lane), to_frag<T>(x[0], e), o[0]);
-                    if (kb == qb && any_nan(o)) {
-                        clear(o);
-                        accumulate_seen<T, DP>(lds_v, 32 * kb, 32 * wave, x[0], [&](int r) { return (lane & 31) >= r; }, o, lane);
-                    }
                 }
                 // what came before it
 #pragma unroll
@@ -190,6 +200,11 @@ __global__ __launch_bounds__(2 * DP, 1) void linear_kernel(LinearParams p) {
                 const float f = qb ? q_decay1 : q_decay0;
 #pragma unroll
                 for (int i = 0; i < 16; ++i) o[0][i] += y[0][i] * f;
+                if (__any(bad < C)) {
+#pragma unroll
+                    for (int i = 0; i < 16; ++i)
+                        if (__shfl(bad, row_of(i, h)) <= 32 * qb + (lane & 31)) o[0][i] = __builtin_nanf("");
+                }
                 const int at = c0 + 32 * qb + (lane & 31);
                 if (at < g.count) {
                     const int64_t token = g.start + (m.reverse ? g.length - 1 - g.first - at : g.first + at);
@@ -223,6 +238,12 @@ __global__ __launch_bounds__(2 * DP, 1) void linear_kernel(LinearParams p) {
             for (int b = 0; b < DB; ++b)
 #pragma unroll
                 for (int i = 0; i < 16; ++i) s[b][i] += low[b][i] * (1.f / 2048.f);
+        }
+        if (__any(bad < C)) {
+#pragma unroll
+            for (int b = 0; b < DB; ++b)
+#pragma unroll
+                for (int i = 0; i < 16; ++i) s[b][i] = bad < C ? __builtin_nanf("") : s[b][i];
         }
         if (!m.shift) {
             const float g1 = exp2_(ld);
