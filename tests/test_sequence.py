@@ -208,7 +208,7 @@ def test_host_layer_refuses_shapes_and_types():
 
 def lists(monkeypatch, lens):
     seqs = sequence.Packed(lens, "cuda:0")
-    monkeypatch.setattr(seqs, "_kept", lambda key, make: list(make()) + [None])
+    monkeypatch.setattr(seqs, "_kept", lambda key, make: list(make()))
     return seqs
 
 
