@@ -116,6 +116,21 @@ template <typename T, int DP> struct Tile {
     }
 };
 
+// acc += A B over DP / 16 steps: A's fragments from `a(step)`, all asked of LDS before the first product waits for one (left to itself the compiler asks for each
+// right before its use, and the matrix pipe idles for an LDS round trip every time)
+template <typename T, int NS, typename A> __device__ __forceinline__ void mma_rows(A a, const frag<T> (&b)[NS], f32x16 &acc) {
+    constexpr int AHEAD = sizeof(T) == 2 ? NS : 2;
+#pragma unroll
+    for (int s0 = 0; s0 < NS; s0 += AHEAD) {
+        frag<T> f[AHEAD];
+#pragma unroll
+        for (int s = 0; s < AHEAD; ++s) f[s] = a(s0 + s);
+        __builtin_amdgcn_sched_barrier(0);
+#pragma unroll
+        for (int s = 0; s < AHEAD; ++s) acc = mma(f[s], b[s0 + s], acc);
+    }
+}
+
 // ---- Global memory.  A buffer descriptor covers the rows of one tile that exist; what lies outside reads as zero, so no lane branches and padding rows and
 // padding columns cost nothing.  The base is 64 bits and moves with the tile, offsets inside it are 32.
 typedef __amdgpu_buffer_rsrc_t rsrc;
@@ -124,6 +139,7 @@ __device__ __forceinline__ rsrc rows_of(const void *base, int rows, uint32_t str
     return __builtin_amdgcn_make_buffer_rsrc((void *)base, 0, n, 0x00020000);
 }
 __device__ __forceinline__ u32x4 load16(rsrc r, uint32_t off) { return __builtin_bit_cast(u32x4, __builtin_amdgcn_raw_buffer_load_b128(r, off, 0, 0)); }
+__device__ __forceinline__ float load4(rsrc r, uint32_t off) { return __builtin_bit_cast(float, __builtin_amdgcn_raw_buffer_load_b32(r, off, 0, 0)); }
 constexpr uint32_t OUTSIDE = 0x80000000u;      // an offset no descriptor reaches (tiles stay below 2 GiB)
 
 // a tile of ROWS rows in the registers of NT threads, on its way from global memory to LDS

@@ -34,127 +34,106 @@ __device__ __forceinline__ float decay2(const float *log_decay, int head) {
     return x < -1e30f ? -1e30f : x;
 }
 
-// Register i of this lane's part of the state: S[32 b + row_of(i, h)][32 wave + l % 32], block b of the key dimension
-template <int DP> __device__ __forceinline__ void state_at(int b, int i, int lane, int wave, int &r, int &c) {
-    r = 32 * b + row_of(i, lane >> 5);
-    c = 32 * wave + (lane & 31);
-}
-
-// acc[b] += K^T (V * tail): the chunk's part of the state.  tail decays per token, so V * tail has float32's 24 bits; it goes through the 16-bit product
-// in parts that add up to it, and the state stays as exact as float32 sums: bf16 in three parts of 8 bits; fp16 in two of 11 (the second scaled by
-// 2^11, with a sum of its own, so that small values do not fall below fp16's range).
-template <int DP, int NB> __device__ __forceinline__ void add_outer(const char *lds_k, int s, f32x8 x, f32x16 (&acc)[NB], f32x16 (&)[NB], int lane, float) {
-#pragma unroll
-    for (int b = 0; b < NB; ++b) acc[b] = mma(Tile<float, DP>::cols(lds_k, 16 * s, 32 * b, lane), x, acc[b]);
-}
-template <int DP, int NB> __device__ __forceinline__ void add_outer(const char *lds_k, int s, f32x8 x, f32x16 (&acc)[NB], f32x16 (&)[NB], int lane, bf16) {
-    bf16x8 p[3];
-#pragma unroll
-    for (int n = 0; n < 3; ++n)
+// acc[b] += K^T (V * tail), a chunk's part of the state.  tail decays per token, so V * tail has float32's 24 bits; it goes through the 16-bit product in
+// parts that add up to it, and the state stays as exact as float32 sums: bf16 in three parts of 8 bits; fp16 in two of 11 (the second scaled by 2^11, with
+// a sum of its own, so that small values do not fall below fp16's range).
+template <typename T, int DP, int C> __device__ __forceinline__ void add_outer(const char *lds_k, const char *lds_v, const float *tail, int col0, f32x16 (&acc)[DP / 32], int lane) {
+    typedef Tile<T, DP> tile;
+    constexpr int E = C / 16, PARTS = sizeof(T) == 4 ? 1 : __is_same(T, f16) ? 2 : 3;
+    auto parts = [&](int e, frag<T> (&p)[PARTS]) {
+        const frag<T> v = tile::cols(lds_v, 16 * e, col0, lane);
+        const f32x4 t0 = *(const f32x4 *)(tail + 16 * e + 4 * (lane >> 5)), t1 = *(const f32x4 *)(tail + 16 * e + 8 + 4 * (lane >> 5));
 #pragma unroll
         for (int j = 0; j < 8; ++j) {
-            p[n][j] = (bf16)x[j];
-            x[j] -= (float)p[n][j];
+            float x = (float)v[j] * (j < 4 ? t0[j % 4] : t1[j % 4]);
+            // x is one float32 from here on: a multiplication fused into one of its uses and not into the other rounds them apart on a tie
+            asm("" : "+v"(x));
+#pragma unroll
+            for (int n = 0; n < PARTS; ++n) {
+                p[n][j] = (T)x;
+                x -= (float)p[n][j];
+                if (__is_same(T, f16)) x *= 2048.f;
+            }
         }
+    };
+    if constexpr (PARTS == 2) {
+        frag<T> p[E][PARTS];
 #pragma unroll
-    for (int b = 0; b < NB; ++b) {
-        bf16x8 k = Tile<bf16, DP>::cols(lds_k, 16 * s, 32 * b, lane);
+        for (int e = 0; e < E; ++e) parts(e, p[e]);
 #pragma unroll
-        for (int n = 2; n >= 0; --n) acc[b] = mma(k, p[n], acc[b]);
-    }
-}
-template <int DP, int NB> __device__ __forceinline__ void add_outer(const char *lds_k, int s, f32x8 x, f32x16 (&acc)[NB], f32x16 (&low)[NB], int lane, f16) {
-    f16x8 p, q;
+        for (int b = 0; b < DP / 32; ++b) {
+            f32x16 low[1];
+            clear(low);
 #pragma unroll
-    for (int j = 0; j < 8; ++j) {
-        // x is one float32 from here on: a multiplication fused into one of its two uses and not into the other rounds them apart on a tie
-        asm("" : "+v"(x[j]));
-        p[j] = (f16)x[j];
-        q[j] = (f16)((x[j] - (float)p[j]) * 2048.f);
-    }
+            for (int e = 0; e < E; ++e) {
+                const frag<T> k = tile::cols(lds_k, 16 * e, 32 * b, lane);
+                acc[b] = mma(k, p[e][0], acc[b]);
+                low[0] = mma(k, p[e][1], low[0]);
+            }
+            acc[b] += low[0] * (1.f / 2048.f);
+        }
+    } else {
 #pragma unroll
-    for (int b = 0; b < NB; ++b) {
-        f16x8 k = Tile<f16, DP>::cols(lds_k, 16 * s, 32 * b, lane);
-        acc[b] = mma(k, p, acc[b]);
-        low[b] = mma(k, q, low[b]);
+        for (int e = 0; e < E; ++e) {
+            frag<T> p[PARTS], k[DP / 32];
+#pragma unroll
+            for (int b = 0; b < DP / 32; ++b) k[b] = tile::cols(lds_k, 16 * e, 32 * b, lane);
+            __builtin_amdgcn_sched_barrier(0);
+            parts(e, p);
+            // (the same block's sums apart: a product does not wait for the one before it)
+#pragma unroll
+            for (int n = PARTS - 1; n >= 0; --n)
+#pragma unroll
+                for (int b = 0; b < DP / 32; ++b) acc[b] = mma(k[b], p[n], acc[b]);
+        }
     }
 }
 
-// A segment of one sequence and head in chunks of 64 tokens.  A wavefront owns 32 columns of the value dimension: DP / 32 of them share the chunk's Q, K and V
-// tiles in LDS and each holds its columns of the state, float32, in registers.  Per chunk: P^T = K Q^T with the decays (every wavefront makes it for
-// itself: cheaper than a turn through LDS), O^T = V^T P^T, plus S^T Q^T with S as the operand it already is, then the state's update.  P and S are rounded
-// to the inputs' type for their products, the state itself never is.
+// A segment of one sequence and head in chunks of C tokens.  For every 32 columns of the value dimension there are two wavefronts, on one SIMD, with about
+// the same number of matrix instructions each: one holds the columns of the state, float32, in registers and updates them (K^T V with the decays); the
+// other makes the outputs from the state before the chunk (P^T = K Q^T with the decays, O^T = V^T P^T + S^T Q^T), which the first leaves for it in LDS as
+// the operand it will be.  One wavefront for both would need more registers than two on a SIMD can have, and then nothing hides its waits.
+// P and S are rounded to the inputs' type for their products, the state itself never is.
 // STATES: only the state that the segment makes from nothing, for `carry`.
+template <typename T> constexpr int chunk_of = sizeof(T) == 4 ? 32 : 64;        // (float32: the tiles and the state's copy have to fit 160 KB of LDS)
 template <typename T, int DP, bool STATES>
-__global__ __launch_bounds__(2 * DP, 1) void linear_kernel(LinearParams p) {
+__global__ __launch_bounds__(STATES ? 2 * DP : 4 * DP, 2) void linear_kernel(LinearParams p) {
     typedef Tile<T, DP> tile;
-    constexpr int C = 64, NT = 2 * DP, NS = DP / 16, DB = DP / 32;
+    constexpr int C = chunk_of<T>, NT = STATES ? 2 * DP : 4 * DP, NS = DP / 16, DB = DP / 32, QB = C / 32;
     __shared__ __attribute__((aligned(16))) char lds_k[C * tile::ROW], lds_v[C * tile::ROW], lds_q[STATES ? 16 : C * tile::ROW];
+    __shared__ __attribute__((aligned(16))) char lds_s[STATES ? 16 : DP * tile::ROW];      // the state before the chunk, transposed
+    __shared__ __attribute__((aligned(16))) float tail[C], to_end[32];      // decay from each token to the last of the chunk; of 32 tokens
+    __shared__ int first_bad[DP];
     __shared__ int nonfinite;        // the chunk (its first token) whose V holds something not finite
     const LinearMode m = p.mode[blockIdx.z];
-    const int head = blockIdx.y, t = threadIdx.x, lane = t & 63, wave = __builtin_amdgcn_readfirstlane(t >> 6), h = lane >> 5, d = p.dim;
+    const int head = blockIdx.y, t = threadIdx.x, lane = t & 63, wave = __builtin_amdgcn_readfirstlane(t >> 6), slice = wave % DB, h = lane >> 5, d = p.dim;
+    const bool keeper = STATES || wave >= DB;       // of the state; else: makes the outputs
     const taco_seq_segment g = p.segments[blockIdx.x];
+    if (STATES && g.first + g.count == g.length) return;        // (nothing starts from the last segment's state)
     const uint32_t rb = d * sizeof(T);
     const float ld = decay2(p.log_decay, head);
     float *carry = p.carry ? p.carry + (((int64_t)blockIdx.z * p.n_segments + blockIdx.x) * p.heads + head) * DP * DP : nullptr;
-
-    f32x16 s[DB];
-    clear(s);
-    if (!STATES) {
-        if (carry) {
-#pragma unroll
-            for (int b = 0; b < DB; ++b)
-#pragma unroll
-                for (int i = 0; i < 16; ++i) {
-                    int r, c;
-                    state_at<DP>(b, i, lane, wave, r, c);
-                    s[b][i] = carry[r * DP + c];
-                }
-        } else if (m.s0) {
-            const float *s0 = m.s0 + ((int64_t)g.sequence * p.heads + head) * d * d;
-#pragma unroll
-            for (int b = 0; b < DB; ++b)
-#pragma unroll
-                for (int i = 0; i < 16; ++i) {
-                    int r, c;
-                    state_at<DP>(b, i, lane, wave, r, c);
-                    s[b][i] = r < d && c < d ? s0[m.transposed ? c * d + r : r * d + c] * m.s0_scale : 0.f;
-                }
-        }
-    }
-    // decays inside a chunk: from key to query (the two blocks of a 32 x 32 triangle's kinds), and to the state behind it
-    float w0[16], w1[16];
-    if (!STATES) {
-#pragma unroll
-        for (int i = 0; i < 16; ++i) {
-            int n = (lane & 31) - row_of(i, h);
-            w0[i] = n >= 0 ? exp2_(ld * n) : 0.f;
-            w1[i] = exp2_(ld * (n + 32));
-        }
-    }
-    const float q_decay0 = exp2_(ld * ((lane & 31) + m.shift)), q_decay1 = exp2_(ld * ((lane & 31) + 32 + m.shift));
+    const int col = 32 * slice + (lane & 31);       // this lane's value dimension
 
     Staged<T, DP, C, NT> sk, sv, sq;
     auto fetch = [&](int c) {
         const int n = min(C, g.count - c), f = g.first + c;
         const int64_t at = g.start + (m.reverse ? g.length - f - n : f);
         rsrc rk = rows_of(m.k.p + at * m.k.ts + head * m.k.hs, n, m.k.ts, rb), rv = rows_of(m.v.p + at * m.v.ts + head * m.v.hs, n, m.v.ts, rb);
+        rsrc rq = rk;
+        if (!STATES) rq = rows_of(m.q.p + at * m.q.ts + head * m.q.hs, n, m.q.ts, rb);
         if (m.reverse) {
             sk.load_reversed(rk, m.k.ts, d, n - 1, t);
             sv.load_reversed(rv, m.v.ts, d, n - 1, t);
+            if (!STATES) sq.load_reversed(rq, m.q.ts, d, n - 1, t);
         } else {
             sk.load(rk, m.k.ts, d, t);
             sv.load(rv, m.v.ts, d, t);
-        }
-        if (!STATES) {
-            rsrc rq = rows_of(m.q.p + at * m.q.ts + head * m.q.hs, n, m.q.ts, rb);
-            if (m.reverse) sq.load_reversed(rq, m.q.ts, d, n - 1, t);
-            else sq.load(rq, m.q.ts, d, t);
+            if (!STATES) sq.load(rq, m.q.ts, d, t);
         }
     };
-    if (g.count > 0) fetch(0);
-    if (t == 0) nonfinite = -1;
-    for (int c0 = 0; c0 < g.count; c0 += C) {
+    // the next chunk into LDS: `leave` between the barriers
+    auto advance = [&](int c0, auto leave) {
         const int n = min(C, g.count - c0);
         __syncthreads();
         if (!STATES && __any(sv.any_nonfinite())) {
@@ -164,46 +143,139 @@ __global__ __launch_bounds__(2 * DP, 1) void linear_kernel(LinearParams p) {
         sk.put(lds_k, t);
         sv.put(lds_v, t);
         if (!STATES) sq.put(lds_q, t);
+        if (n < C && t < C) tail[t] = exp2_(ld * max(n - 1 - t, 0));     // (behind the last token: v = 0)
+        leave();
         __syncthreads();
-        int bad = C;        // the first token of the chunk whose V is not finite in this lane's column
-        if (!STATES && nonfinite == c0) {
-            const int col = 32 * wave + (lane & 31), f = g.first + c0;
-            const char *v = m.v.p + (g.start + (m.reverse ? g.length - 1 - f : f)) * m.v.ts + head * m.v.hs;
-            int plus, minus;
-            first_nonfinite<T>(v, m.reverse ? -m.v.ts : m.v.ts, col < d ? n : 0, col < d ? col : 0, plus, minus);
-            if (col < d && min(plus, minus) < n) bad = min(plus, minus);
-        }
         if (c0 + C < g.count) fetch(c0 + C);
+        return n;
+    };
+    // the first token of the chunk whose V is not finite in this lane's column (C: none)
+    auto first_nonfinite_token = [&](int c0, int n) {
+        const int f = g.first + c0;
+        const char *v = m.v.p + (g.start + (m.reverse ? g.length - 1 - f : f)) * m.v.ts + head * m.v.hs;
+        int plus, minus;
+        first_nonfinite<T>(v, m.reverse ? -m.v.ts : m.v.ts, col < d ? n : 0, col < d ? col : 0, plus, minus);
+        return col < d && min(plus, minus) < n ? min(plus, minus) : C;
+    };
+    if (g.count > 0) fetch(0);
+    if (t == 0) nonfinite = -1;
+    if (t < C) tail[t] = exp2_(ld * (C - 1 - t));
+    if (t < 32) to_end[t] = exp2_(ld * (31 - t));
+
+    if (keeper) {
+        f32x16 s[DB];
+        clear(s);
         if (!STATES) {
+            const float *from = carry ? carry : m.s0 ? m.s0 + ((int64_t)g.sequence * p.heads + head) * d * d : nullptr;
+            const int size = carry ? DP : d;
+            const bool turned = !carry && m.transposed;
+            const float f = carry ? 1.f : m.s0_scale;
+            // (through a descriptor: outside reads as zero, and all loads are on their way at once)
+            const rsrc state = rows_of(from, from ? 1 : 0, 0, size * size * 4);
 #pragma unroll
-            for (int qb = 0; qb < 2; ++qb) {
+            for (int b = 0; b < DB; ++b)
+#pragma unroll
+                for (int i = 0; i < 16; ++i) {
+                    const int r = 32 * b + row_of(i, h);
+                    s[b][i] = load4(state, r < size && col < size ? (turned ? col * size + r : r * size + col) * 4 : OUTSIDE);
+                }
+#pragma unroll
+            for (int b = 0; b < DB; ++b) s[b] *= f;
+        }
+        for (int c0 = 0; c0 < g.count; c0 += C) {
+            const int n = advance(c0, [&]() {
+                if constexpr (!STATES) {
+#pragma unroll
+                    for (int b = 0; b < DB; ++b)
+#pragma unroll
+                        for (int i = 0; i < 16; i += 4) {
+                            const int r = 32 * b + row_of(i, h);
+                            store4((T *)(lds_s + tile::at(col, r / tile::CE) + r % tile::CE * (int)sizeof(T)), s[b][i], s[b][i + 1], s[b][i + 2], s[b][i + 3]);
+                        }
+                }
+            });
+            // (shift 0: the chunk's own part decays once more, behind its product: a strong decay would leave nothing of it in fp16)
+            const float gn = exp2_(ld * (n - 1 + m.shift));
+#pragma unroll
+            for (int b = 0; b < DB; ++b) s[b] *= gn;
+            add_outer<T, DP, C>(lds_k, lds_v, tail, 32 * slice, s, lane);
+            if (!STATES && nonfinite == c0) {
+                const bool bad = first_nonfinite_token(c0, n) < C;
+#pragma unroll
+                for (int b = 0; b < DB; ++b) s[b] += bad ? __builtin_nanf("") : 0.f;
+            }
+            if (!m.shift) {
+                const float g1 = exp2_(ld);
+#pragma unroll
+                for (int b = 0; b < DB; ++b) s[b] *= g1;
+            }
+        }
+        if (STATES) {
+#pragma unroll
+            for (int b = 0; b < DB; ++b)
+#pragma unroll
+                for (int i = 0; i < 16; ++i) carry[(32 * b + row_of(i, h)) * DP + col] = s[b][i];
+        } else if (m.last && g.first + g.count == g.length && (g.count > 0 || g.length == 0)) {
+            float *out = m.last + ((int64_t)g.sequence * p.heads + head) * d * d;
+#pragma unroll
+            for (int b = 0; b < DB; ++b)
+#pragma unroll
+                for (int i = 0; i < 16; ++i) {
+                    const int r = 32 * b + row_of(i, h);
+                    if (r < d && col < d) out[r * d + col] = s[b][i] * m.last_scale;
+                }
+        }
+        return;
+    }
+    if constexpr (!STATES) {
+        // decay from key to query inside a block of 32; from an earlier block: the key's to that block's end (to_end), then this lane's query's from there
+        float w0[16];
+#pragma unroll
+        for (int i = 0; i < 16; ++i) {
+            const int n = (lane & 31) - row_of(i, h);
+            w0[i] = n >= 0 ? exp2_(ld * n) : 0.f;
+        }
+        const float q_entry = exp2_(ld * ((lane & 31) + 1));
+        for (int c0 = 0; c0 < g.count; c0 += C) {
+            const int n = advance(c0, []() {});
+            const bool bad = nonfinite == c0;
+            if (bad) {
+                first_bad[col] = first_nonfinite_token(c0, n);      // (both halves of the wavefront write the same)
+                __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
+            }
+#pragma unroll
+            for (int qb = 0; qb < QB; ++qb) {
                 if (32 * qb >= n) continue;
+                frag<T> qf[NS];
+#pragma unroll
+                for (int e = 0; e < NS; ++e) qf[e] = tile::rows(lds_q, 32 * qb, e, lane);
                 f32x16 o[1], x[1], y[1];
                 clear(o);
                 clear(y);
+                // what came before the chunk
+                mma_rows<T>([&](int e) { return tile::rows(lds_s, 32 * slice, e, lane); }, qf, y[0]);
                 // the chunk itself
 #pragma unroll
                 for (int kb = qb; kb >= 0; --kb) {
+                    frag<T> vf[2];
                     clear(x);
+                    mma_rows<T>([&](int e) { return tile::rows(lds_k, 32 * kb, e, lane); }, qf, x[0]);
 #pragma unroll
-                    for (int e = 0; e < NS; ++e) x[0] = mma(tile::rows(lds_k, 32 * kb, e, lane), tile::rows(lds_q, 32 * qb, e, lane), x[0]);
+                    for (int e = 0; e < 2; ++e) vf[e] = tile::cols(lds_v, 32 * kb + 16 * e, 32 * slice, lane);
 #pragma unroll
-                    for (int i = 0; i < 16; ++i) x[0][i] = kb == qb ? ((lane & 31) >= row_of(i, h) ? x[0][i] * w0[i] : 0.f) : x[0][i] * w1[i];
+                    for (int i = 0; i < 16; i += 4) {
+                        const f32x4 w = *(const f32x4 *)(to_end + row_of(i, h));
 #pragma unroll
-                    for (int e = 0; e < 2; ++e) o[0] = mma(tile::cols(lds_v, 32 * kb + 16 * e, 32 * wave, lane), to_frag<T>(x[0], e), o[0]);
+                        for (int j = 0; j < 4; ++j)
+                            x[0][i + j] = kb == qb ? ((lane & 31) >= row_of(i + j, h) ? x[0][i + j] * w0[i + j] : 0.f) : x[0][i + j] * (w[j] * q_entry);
+                    }
+#pragma unroll
+                    for (int e = 0; e < 2; ++e) o[0] = mma(vf[e], to_frag<T>(x[0], e), o[0]);
                 }
-                // what came before it
+                o[0] += y[0] * exp2_(ld * (32 * qb + (lane & 31) + m.shift));
+                if (bad) {
 #pragma unroll
-                for (int b = 0; b < DB; ++b)
-#pragma unroll
-                    for (int e = 0; e < 2; ++e) y[0] = mma(to_frag<T>(s[b], e), tile::rows_permuted(lds_q, 32 * qb, 32 * b + 16 * e, lane), y[0]);
-                const float f = qb ? q_decay1 : q_decay0;
-#pragma unroll
-                for (int i = 0; i < 16; ++i) o[0][i] += y[0][i] * f;
-                if (__any(bad < C)) {
-#pragma unroll
-                    for (int i = 0; i < 16; ++i)
-                        if (__shfl(bad, row_of(i, h)) <= 32 * qb + (lane & 31)) o[0][i] = __builtin_nanf("");
+                    for (int i = 0; i < 16; ++i) o[0][i] = first_bad[32 * slice + row_of(i, h)] <= 32 * qb + (lane & 31) ? __builtin_nanf("") : o[0][i];
                 }
                 const int at = c0 + 32 * qb + (lane & 31);
                 if (at < g.count) {
@@ -211,67 +283,12 @@ __global__ __launch_bounds__(2 * DP, 1) void linear_kernel(LinearParams p) {
                     T *row = (T *)(m.o.p + token * m.o.ts + head * m.o.hs);
 #pragma unroll
                     for (int i = 0; i < 16; i += 4) {
-                        const int c = 32 * wave + row_of(i, h);
+                        const int c = 32 * slice + row_of(i, h);
                         if (c < d) store4(row + c, o[0][i] * m.scale, o[0][i + 1] * m.scale, o[0][i + 2] * m.scale, o[0][i + 3] * m.scale);
                     }
                 }
             }
         }
-        // (shift 0: the chunk's own part decays once more, behind its product: a strong decay would leave nothing of it in fp16)
-        const float gn = exp2_(ld * (n - 1 + m.shift));
-        f32x16 low[DB];
-        clear(low);
-#pragma unroll
-        for (int b = 0; b < DB; ++b)
-#pragma unroll
-            for (int i = 0; i < 16; ++i) s[b][i] *= gn;
-#pragma unroll
-        for (int e = 0; e < C / 16; ++e) {
-            frag<T> v = tile::cols(lds_v, 16 * e, 32 * wave, lane);
-            f32x8 x;
-#pragma unroll
-            for (int j = 0; j < 8; ++j) x[j] = (float)v[j] * exp2_(ld * max(n - 1 - 16 * e - row_of(j, h), 0));      // (behind the last token: v = 0)
-            add_outer<DP>(lds_k, e, x, s, low, lane, T());
-        }
-        if (__is_same(T, f16)) {
-#pragma unroll
-            for (int b = 0; b < DB; ++b)
-#pragma unroll
-                for (int i = 0; i < 16; ++i) s[b][i] += low[b][i] * (1.f / 2048.f);
-        }
-        if (__any(bad < C)) {
-#pragma unroll
-            for (int b = 0; b < DB; ++b)
-#pragma unroll
-                for (int i = 0; i < 16; ++i) s[b][i] = bad < C ? __builtin_nanf("") : s[b][i];
-        }
-        if (!m.shift) {
-            const float g1 = exp2_(ld);
-#pragma unroll
-            for (int b = 0; b < DB; ++b)
-#pragma unroll
-                for (int i = 0; i < 16; ++i) s[b][i] *= g1;
-        }
-    }
-    if (STATES) {
-#pragma unroll
-        for (int b = 0; b < DB; ++b)
-#pragma unroll
-            for (int i = 0; i < 16; ++i) {
-                int r, c;
-                state_at<DP>(b, i, lane, wave, r, c);
-                carry[r * DP + c] = s[b][i];
-            }
-    } else if (m.last && g.first + g.count == g.length && (g.count > 0 || g.length == 0)) {
-        float *out = m.last + ((int64_t)g.sequence * p.heads + head) * d * d;
-#pragma unroll
-        for (int b = 0; b < DB; ++b)
-#pragma unroll
-            for (int i = 0; i < 16; ++i) {
-                int r, c;
-                state_at<DP>(b, i, lane, wave, r, c);
-                if (r < d && c < d) out[r * d + c] = s[b][i] * m.last_scale;
-            }
     }
 }
 
@@ -283,7 +300,7 @@ template <int DP> __global__ __launch_bounds__(256) void linear_scan_kernel(Line
     float s = m.s0 && r < d && c < d ? m.s0[((int64_t)seq * p.heads + head) * d * d + (m.transposed ? c * d + r : r * d + c)] * m.s0_scale : 0.f;
     for (int i = p.first_segment[seq]; i < p.first_segment[seq + 1]; ++i) {
         float *x = p.carry + (((int64_t)blockIdx.z * p.n_segments + i) * p.heads + head) * DP * DP + e;
-        const float own = *x;
+        const float own = i + 1 < p.first_segment[seq + 1] ? *x : 0.f;      // (the last segment's is not made, and nothing starts from it)
         *x = s;
         s = s * exp2_(ld * p.segments[i].count) + own;
     }

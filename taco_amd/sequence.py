@@ -237,18 +237,19 @@ class Packed:
         return [got[i:i + 4] for i in range(0, len(got), 4)]
 
     def _segments(self, work):
-        """(segments, first segment of each sequence, count) for `work` = heads x products: about 1 024 workgroups in all, segments of at least 256 tokens"""
-        size = max(256, -(-self.total * work // (1024 * 64)) * 64)
+        """(segments, first segment of each sequence, count) for `work` = heads x products.  A workgroup fills a CU, so pieces of a third of a CU's share of all tokens
+        (at least 256) even out what sequences of different lengths leave; a sequence is cut into equal pieces where it is longer than one and a half."""
+        size = max(256, -(-self.total * work // (768 * 64)) * 64)
         key = ("segments", size)
 
         def make():
-            n = np.maximum(-(-self.lengths // size), 1)
-            if len(n) and n.sum() > len(n) and len(n) * 128 > 65535:       # (the joining launch's limit; so many sequences fill the CUs by themselves)
+            n = np.where(self.lengths <= size + size // 2, 1, -(-self.lengths // size))
+            if len(n) and n.sum() > len(n) and len(n) * work > 65535:      # (the joining launch's limit; so many sequences fill the CUs by themselves)
                 n = np.ones_like(n)
             first = np.concatenate([[0], np.cumsum(n)])
             of = np.repeat(np.arange(len(n)), n)
             index = np.arange(len(of)) - first[of]
-            step = np.where(n[of] > 1, size, self.lengths[of])
+            step = np.where(n[of] > 1, -(-self.lengths[of] // (n[of] * 64)) * 64, self.lengths[of])
             at = index * step
             cols = [of, self.starts[of], self.lengths[of], at, np.minimum(step, self.lengths[of] - at), index, index * 0, index * 0]
             return [np.stack(cols, 1).astype(np.int32).reshape(-1, 8), first.astype(np.int32), len(of)]
