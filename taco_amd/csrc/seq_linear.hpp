@@ -249,11 +249,11 @@ __global__ __launch_bounds__(STATES ? 2 * DP : 4 * DP, 2) void linear_kernel(Lin
                 frag<T> qf[NS];
 #pragma unroll
                 for (int e = 0; e < NS; ++e) qf[e] = tile::rows(lds_q, 32 * qb, e, lane);
-                f32x16 o[1], x[1], y[1];
+                f32x16 o[1], x[1];
                 clear(o);
-                clear(y);
                 // what came before the chunk
-                mma_rows<T>([&](int e) { return tile::rows(lds_s, 32 * slice, e, lane); }, qf, y[0]);
+                mma_rows<T>([&](int e) { return tile::rows(lds_s, 32 * slice, e, lane); }, qf, o[0]);
+                o[0] *= exp2_(ld * (32 * qb + (lane & 31) + m.shift));
                 // the chunk itself
 #pragma unroll
                 for (int kb = qb; kb >= 0; --kb) {
@@ -272,7 +272,6 @@ __global__ __launch_bounds__(STATES ? 2 * DP : 4 * DP, 2) void linear_kernel(Lin
 #pragma unroll
                     for (int e = 0; e < 2; ++e) o[0] = mma(vf[e], to_frag<T>(x[0], e), o[0]);
                 }
-                o[0] += y[0] * exp2_(ld * (32 * qb + (lane & 31) + m.shift));
                 if (bad) {
 #pragma unroll
                     for (int i = 0; i < 16; ++i) o[0][i] = first_bad[32 * slice + row_of(i, h)] <= 32 * qb + (lane & 31) ? __builtin_nanf("") : o[0][i];

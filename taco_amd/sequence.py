@@ -237,9 +237,9 @@ class Packed:
         return [got[i:i + 4] for i in range(0, len(got), 4)]
 
     def _segments(self, work):
-        """(segments, first segment of each sequence, count) for `work` = heads x products.  A workgroup fills a CU, so pieces of a third of a CU's share of all tokens
+        """(segments, first segment of each sequence, count) for `work` = heads x products.  A workgroup fills a CU, so pieces of half a CU's share of all tokens
         (at least 256) even out what sequences of different lengths leave; a sequence is cut into equal pieces where it is longer than one and a half."""
-        size = max(256, -(-self.total * work // (768 * 64)) * 64)
+        size = max(256, -(-self.total * work // (512 * 64)) * 64)
         key = ("segments", size)
 
         def make():
