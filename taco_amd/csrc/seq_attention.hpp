@@ -26,7 +26,17 @@ __device__ __forceinline__ void locate(int block, int heads, int &tile, int &hea
     if (heads % 8 == 0) head = (head % 8) * (heads / 8) + head / 8;
 }
 
-template <typename T> constexpr int waves_per_simd(int nw) { return nw == 4 && sizeof(T) == 2 ? 2 : 1; }
+// Wavefronts per SIMD that the registers are cut for: as many as do not spill.  Nothing else hides the latency of loads and of the chain of products, least
+// of all where a sequence is one tile.
+template <typename T, int DP, int NW> constexpr int waves_forward = sizeof(T) == 4 ? (DP == 32 ? 2 : 1) : DP == 32 ? 4 : DP == 64 || NW == 4 ? 2 : 1;
+template <typename T, int DP> constexpr int waves_backward = sizeof(T) == 4 ? (DP == 32 ? 2 : 1) : DP <= 64 ? 2 : 1;
+// The next tiles travel in registers while these are used, except where that would spill: float32 rows of 128 hold half the registers as operands already.
+template <typename T, int DP> constexpr bool ahead = !(sizeof(T) == 4 && DP == 128);
+
+// (and there the compiler must not ask LDS for many operands at once either)
+template <typename T, int DP> __device__ __forceinline__ void in_order() {
+    if (!ahead<T, DP>) __builtin_amdgcn_sched_barrier(0);
+}
 
 // acc += X w for a product whose tile X of 32 rows is read by columns: one step of a running sum in acc.  float32 sums each tile apart first: the sum over a long
 // sequence then has a rounding per tile in it, not per pair of rows (its error is the float32 result's own; the 16-bit types' roundings are larger).
@@ -42,6 +52,7 @@ template <typename T, int DP> __device__ __forceinline__ void add_columns(const 
 #pragma unroll
             for (int x = 0; x < 2; ++x) y[0] = mma(Tile<T, DP>::cols(lds, row0 + 16 * x, 32 * b, lane), f[x], y[0]);
             acc[b] += y[0];
+            in_order<T, DP>();
         }
     } else {
 #pragma unroll
@@ -57,7 +68,7 @@ template <typename T, int DP> __device__ __forceinline__ void add_columns(const 
 // as much as the output's own rounding); its sum stays float32.
 // Keys run from the diagonal to the first one.  The tiles that hide keys come first, in a loop of their own, and the others run without a mask.
 template <typename T, int DP, int NW>
-__global__ __launch_bounds__(64 * NW, waves_per_simd<T>(NW)) void attention_kernel(AttentionParams p) {
+__global__ __launch_bounds__(64 * NW, (waves_forward<T, DP, NW>)) void attention_kernel(AttentionParams p) {
     typedef Tile<T, DP> tile;
     constexpr int BM = 32 * NW, BN = NW == 1 ? 32 : 64, NB = BN / 32, NS = DP / 16, DB = DP / 32, NT = 64 * NW;
     __shared__ __attribute__((aligned(16))) char lds_k[BN * tile::ROW], lds_v[BN * tile::ROW];
@@ -94,7 +105,10 @@ __global__ __launch_bounds__(64 * NW, waves_per_simd<T>(NW)) void attention_kern
 #pragma unroll
         for (int n = 0; n < NB; ++n)
 #pragma unroll
-            for (int x = 0; x < NS; ++x) s[n] = mma(tile::rows(lds_k, 32 * n, x, lane), qf[x], s[n]);
+            for (int x = 0; x < NS; ++x) {
+                s[n] = mma(tile::rows(lds_k, 32 * n, x, lane), qf[x], s[n]);
+                in_order<T, DP>();
+            }
     };
     auto softmax = [&](f32x16 (&s)[NB]) {
         float mx = s[0][0];
@@ -125,10 +139,11 @@ __global__ __launch_bounds__(64 * NW, waves_per_simd<T>(NW)) void attention_kern
     int kt = last / BN;
     // tiles from here up hide keys of the sequence from some query of the workgroup (causal), or hold rows behind its end
     const int whole = p.causal ? w.first / BN : w.length / BN;
-    fetch(kt);
+    if (ahead<T, DP>) fetch(kt);
     if (t == 0) nonfinite = 0;
     for (; kt >= whole; --kt) {
         __syncthreads();
+        if (!ahead<T, DP>) fetch(kt);
         const bool bad = p.causal && __any(sv.any_nonfinite());
         if (bad) {
             sv.nonfinite_to_zero();
@@ -137,7 +152,7 @@ __global__ __launch_bounds__(64 * NW, waves_per_simd<T>(NW)) void attention_kern
         sk.put(lds_k, t);
         sv.put(lds_v, t);
         __syncthreads();
-        if (kt > 0) fetch(kt - 1);
+        if (ahead<T, DP> && kt > 0) fetch(kt - 1);
         const int k0 = kt * BN;
         if (p.causal && k0 > first + 31) continue;      // (the wavefront's: all of the tile is hidden)
         f32x16 s[NB];
@@ -171,10 +186,11 @@ __global__ __launch_bounds__(64 * NW, waves_per_simd<T>(NW)) void attention_kern
     }
     for (; kt >= 0; --kt) {
         __syncthreads();
+        if (!ahead<T, DP>) fetch(kt);
         sk.put(lds_k, t);
         sv.put(lds_v, t);
         __syncthreads();
-        if (kt > 0) fetch(kt - 1);
+        if (ahead<T, DP> && kt > 0) fetch(kt - 1);
         f32x16 s[NB];
         scores(s);
         softmax(s);
@@ -194,7 +210,7 @@ __global__ __launch_bounds__(64 * NW, waves_per_simd<T>(NW)) void attention_kern
 // A query that sees few keys has gradients that are small differences of dP and delta, and o as it was rounded would set their error.  Where all its keys
 // lie in one tile, delta is the sum of P dP over that tile instead, in float32.
 template <typename T, int DP, int NW>
-__global__ __launch_bounds__(64 * NW, 1) void attention_dq_kernel(AttentionParams p) {
+__global__ __launch_bounds__(64 * NW, (waves_backward<T, DP>)) void attention_dq_kernel(AttentionParams p) {
     typedef Tile<T, DP> tile;
     constexpr int BM = 32 * NW, BN = NW == 1 ? 32 : 64, NB = BN / 32, NS = DP / 16, DB = DP / 32, NT = 64 * NW;
     __shared__ __attribute__((aligned(16))) char lds_k[BN * tile::ROW], lds_v[BN * tile::ROW];
@@ -244,19 +260,26 @@ __global__ __launch_bounds__(64 * NW, 1) void attention_dq_kernel(AttentionParam
         f32x16 x[2];
         clear(x);
 #pragma unroll
-        for (int y = 0; y < NS; ++y) x[0] = mma(tile::rows(lds_k, 32 * n, y, lane), qf[y], x[0]);
+        for (int y = 0; y < NS; ++y) {
+            x[0] = mma(tile::rows(lds_k, 32 * n, y, lane), qf[y], x[0]);
+            in_order<T, DP>();
+        }
 #pragma unroll
-        for (int y = 0; y < NS; ++y) x[1] = mma(tile::rows(lds_v, 32 * n, y, lane), gf[y], x[1]);
+        for (int y = 0; y < NS; ++y) {
+            x[1] = mma(tile::rows(lds_v, 32 * n, y, lane), gf[y], x[1]);
+            in_order<T, DP>();
+        }
 #pragma unroll
         for (int i = 0; i < 16; ++i) pr[i] = exp2_(x[0][i] * c - mu);
         dp = x[1];
     };
     int kt = last / BN;
     const int whole = p.causal ? w.first / BN : w.length / BN;
-    fetch(kt);
+    if (ahead<T, DP>) fetch(kt);
     if (t == 0) nonfinite = BN;
     for (; kt >= whole; --kt) {
         __syncthreads();
+        if (!ahead<T, DP>) fetch(kt);
         if (p.causal && __any(sk.any_nonfinite())) {
             int r = BN;
 #pragma unroll
@@ -269,7 +292,7 @@ __global__ __launch_bounds__(64 * NW, 1) void attention_dq_kernel(AttentionParam
         sv.put(lds_v, t);
         __syncthreads();
         const int seen_bad = nonfinite;
-        if (kt > 0) fetch(kt - 1);
+        if (ahead<T, DP> && kt > 0) fetch(kt - 1);
         const int k0 = kt * BN;
         if (!(p.causal && k0 > first + 31)) {      // (else: all of the tile is hidden from the wavefront)
             f32x16 pr[NB], ds[NB];
@@ -309,10 +332,11 @@ __global__ __launch_bounds__(64 * NW, 1) void attention_dq_kernel(AttentionParam
     }
     for (; kt >= 0; --kt) {
         __syncthreads();
+        if (!ahead<T, DP>) fetch(kt);
         sk.put(lds_k, t);
         sv.put(lds_v, t);
         __syncthreads();
-        if (kt > 0) fetch(kt - 1);
+        if (ahead<T, DP> && kt > 0) fetch(kt - 1);
 #pragma unroll
         for (int n = 0; n < NB; ++n) {
             f32x16 pr, ds;
@@ -332,7 +356,7 @@ __global__ __launch_bounds__(64 * NW, 1) void attention_dq_kernel(AttentionParam
 // for every query head of the group in turn, so the gradients of a shared head are sums in registers.  S = Q K^T and dP = dO V^T have the keys in
 // the lanes; P and dS are the operands of dV^T = dO^T P and dK^T = Q^T dS as they stand.
 template <typename T, int DP, int NW>
-__global__ __launch_bounds__(64 * NW, 1) void attention_dkv_kernel(AttentionParams p) {
+__global__ __launch_bounds__(64 * NW, (waves_backward<T, DP>)) void attention_dkv_kernel(AttentionParams p) {
     typedef Tile<T, DP> tile;
     constexpr int BK = 32 * NW, BQ = NW == 1 ? 32 : 64, NB = BQ / 32, NS = DP / 16, DB = DP / 32, NT = 64 * NW;
     __shared__ __attribute__((aligned(16))) char lds_q[BQ * tile::ROW], lds_g[BQ * tile::ROW];
@@ -388,9 +412,15 @@ __global__ __launch_bounds__(64 * NW, 1) void attention_dkv_kernel(AttentionPara
     auto weights = [&](int n, f32x16 (&x)[2]) {
         clear(x);
 #pragma unroll
-        for (int y = 0; y < NS; ++y) x[0] = mma(tile::rows(lds_q, 32 * n, y, lane), kf[y], x[0]);
+        for (int y = 0; y < NS; ++y) {
+            x[0] = mma(tile::rows(lds_q, 32 * n, y, lane), kf[y], x[0]);
+            in_order<T, DP>();
+        }
 #pragma unroll
-        for (int y = 0; y < NS; ++y) x[1] = mma(tile::rows(lds_g, 32 * n, y, lane), vf[y], x[1]);
+        for (int y = 0; y < NS; ++y) {
+            x[1] = mma(tile::rows(lds_g, 32 * n, y, lane), vf[y], x[1]);
+            in_order<T, DP>();
+        }
 #pragma unroll
         for (int i = 0; i < 16; i += 4) {
             f32x4 mu = *(const f32x4 *)(lds_mu + 32 * n + row_of(i, h)), de = *(const f32x4 *)(lds_delta + 32 * n + row_of(i, h));
@@ -401,16 +431,18 @@ __global__ __launch_bounds__(64 * NW, 1) void attention_dkv_kernel(AttentionPara
             }
         }
     };
-    fetch(kvh * G, qt0);
+    if (ahead<T, DP>) fetch(kvh * G, qt0);
     if (t == 0) nonfinite = -1;
     for (int head = kvh * G; head < (kvh + 1) * G; ++head) {
         int qt = qt0;
         auto next = [&]() {
+            if (!ahead<T, DP>) return;
             if (qt + 1 < qt1) fetch(head, qt + 1);
             else if (head + 1 < (kvh + 1) * G) fetch(head + 1, qt0);
         };
         for (; qt < whole; ++qt) {
             __syncthreads();
+            if (!ahead<T, DP>) fetch(head, qt);
             if (__any(sq.any_nonfinite() || sg.any_nonfinite())) {
                 int r = -1;
 #pragma unroll
@@ -451,6 +483,7 @@ __global__ __launch_bounds__(64 * NW, 1) void attention_dkv_kernel(AttentionPara
         }
         for (; qt < qt1; ++qt) {
             __syncthreads();
+            if (!ahead<T, DP>) fetch(head, qt);
             put();
             __syncthreads();
             next();
