@@ -49,6 +49,7 @@ typedef struct taco_attention_args {
     const taco_seq_tile *tiles;
     const taco_seq_tile *key_tiles;     /* backward: the same tiles in the order their keys want (most queries first), or NULL */
     int32_t n_tiles, tile_rows;
+    int32_t whole;                      /* not 0: every tile is a whole sequence, of at most tile_rows = 32 tokens (longer ones are cut off there) */
     int32_t heads, kv_heads, dim, dtype, causal;
     float scale;                        /* > 0 */
     /* backward only: */
@@ -56,7 +57,8 @@ typedef struct taco_attention_args {
     float *delta;                       /* workspace [tokens][heads] */
 } taco_attention_args;
 int taco_attention(const taco_attention_args *a, void *stream);
-/* Gradients by the formulas (P from lse; dS = P (dP - rowsum(d_o o))): two launches, the second reads `delta`, which the first writes. */
+/* Gradients by the formulas (P from lse; dS = P (dP - rowsum(d_o o))): two launches, the second reads `delta`, which the first writes; one launch where
+ * the tiles are whole sequences (o and delta are not read then). */
 int taco_attention_backward(const taco_attention_args *a, void *stream);
 
 /* ---- Attention of one new token per row over a paged cache, which the token joins.

@@ -502,4 +502,121 @@ __global__ __launch_bounds__(64 * NW, (waves_backward<T, DP>)) void attention_dk
     }
 }
 
+// Backward of sequences of at most 32 tokens, all of it: one wavefront for a sequence and a key-value head.  S and dP are made once (five products), delta is the
+// sum of P dP, and dK and dV take P and dS turned around through LDS (a wavefront's own, no barrier).  q, k, v, d_o and lse are read once and the gradients
+// written once, where the two launches above read q, k, v and d_o twice and o as well.  Not for float32 rows of 128: their operands leave no registers.
+template <typename T, int DP> constexpr bool short_gradients = !(sizeof(T) == 4 && DP == 128);
+template <typename T, int DP>
+__global__ __launch_bounds__(64, DP == 32 ? 2 : 1) void attention_short_grad_kernel(AttentionParams p) {
+    typedef Tile<T, DP> tile;
+    typedef Tile<T, 32> square;
+    constexpr int NS = DP / 16, DB = DP / 32;
+    __shared__ __attribute__((aligned(16))) char lds_k[32 * tile::ROW], lds_q[32 * tile::ROW], lds_g[32 * tile::ROW], lds_w[32 * square::ROW];
+    int ti, kvh;
+    locate(blockIdx.x, p.kv_heads, ti, kvh);
+    const taco_seq_tile w = p.key_tiles[ti];
+    const int lane = threadIdx.x, h = lane >> 5, r = lane & 31, d = p.dim, G = p.heads / p.kv_heads, length = min(w.length, 32);
+    const uint32_t rb = d * sizeof(T);
+    const float c = p.scale * LOG2E;
+    const int64_t at = w.start;
+    // the first key, and the last query, with something not finite in its row (a query: or its gradient's); such rows leave the tiles as zeros
+    auto stage = [&](char *lds, rsrc from, uint32_t stride, int &first, int &last) {
+        Staged<T, DP, 32, 64> s;
+        s.load(from, stride, d, lane);
+        if (p.causal && __any(s.any_nonfinite())) {
+#pragma unroll
+            for (int i = 0; i < Staged<T, DP, 32, 64>::N; ++i)
+                if (s.chunk_nonfinite(i)) {
+                    first = min(first, (i * 64 + lane) / tile::NC);
+                    last = max(last, (i * 64 + lane) / tile::NC);
+                }
+#pragma unroll
+            for (int i = 32; i > 0; i >>= 1) {
+                first = min(first, __shfl_xor(first, i));
+                last = max(last, __shfl_xor(last, i));
+            }
+            s.nonfinite_to_zero();
+        }
+        s.put(lds, lane);
+    };
+    int bad_key = 32, unused = -1;
+    stage(lds_k, rows_of(p.k.p + at * p.k.ts + kvh * p.k.hs, length, p.k.ts, rb), p.k.ts, bad_key, unused);
+    frag<T> vf[NS];
+    {
+        const rsrc rv = rows_of(p.v.p + at * p.v.ts + kvh * p.v.hs, length, p.v.ts, rb);
+#pragma unroll
+        for (int s = 0; s < NS; ++s) vf[s] = rows_global<T>(rv, p.v.ts, d, 0, s, lane);
+    }
+    f32x16 dk[DB], dv[DB];
+    clear(dk);
+    clear(dv);
+    int bad_query = -1;
+    for (int head = kvh * G; head < (kvh + 1) * G; ++head) {
+        const rsrc rq = rows_of(p.q.p + at * p.q.ts + head * p.q.hs, length, p.q.ts, rb), rg = rows_of(p.d_o.p + at * p.d_o.ts + head * p.d_o.hs, length, p.d_o.ts, rb);
+        int ignored = 32;
+        __syncthreads();
+        stage(lds_q, rq, p.q.ts, ignored, bad_query);
+        stage(lds_g, rg, p.d_o.ts, ignored, bad_query);
+        const float lse = r < length ? p.lse[(at + r) * p.heads + head] : -__builtin_inff();
+        const float mu = lse == -__builtin_inff() ? __builtin_inff() : lse * LOG2E;
+        __syncthreads();
+        // columns: the queries
+        f32x16 x[2];
+        clear(x);
+#pragma unroll
+        for (int s = 0; s < NS; ++s) x[0] = mma(tile::rows(lds_k, 0, s, lane), rows_global<T>(rq, p.q.ts, d, 0, s, lane), x[0]);
+#pragma unroll
+        for (int s = 0; s < NS; ++s) x[1] = mma(vf[s], rows_global<T>(rg, p.d_o.ts, d, 0, s, lane), x[1]);
+        const int limit = p.causal ? r : length - 1;
+        float delta = 0.f;
+#pragma unroll
+        for (int i = 0; i < 16; ++i) {
+            const bool seen = row_of(i, h) <= limit;
+            x[0][i] = seen ? exp2_(x[0][i] * c - mu) : 0.f;
+            x[1][i] = seen ? x[1][i] : 0.f;
+            delta += x[0][i] * x[1][i];
+        }
+        delta += other_half(delta);
+#pragma unroll
+        for (int i = 0; i < 16; ++i) x[1][i] = row_of(i, h) <= limit ? x[0][i] * (x[1][i] - delta) : 0.f;
+        f32x16 dq[DB];
+        clear(dq);
+        add_columns<T, DP>(lds_k, 0, x[1], dq, lane);
+        if (bad_key <= limit) {
+#pragma unroll
+            for (int b = 0; b < DB; ++b) dq[b] += __builtin_nanf("");
+        }
+        if (r < length) store_row<T>((T *)(p.d_q.p + (at + r) * p.d_q.ts + head * p.d_q.hs), dq, p.scale, d, lane);
+        // columns: the keys
+#pragma unroll
+        for (int y = 0; y < 2; ++y) {
+            __syncthreads();
+#pragma unroll
+            for (int i = 0; i < 16; ++i) *(T *)(lds_w + square::at(row_of(i, h), r / square::CE) + r % square::CE * (int)sizeof(T)) = (T)x[y][i];
+            __syncthreads();
+            frag<T> f[2];
+#pragma unroll
+            for (int s = 0; s < 2; ++s) f[s] = square::rows_permuted(lds_w, 0, 16 * s, lane);
+#pragma unroll
+            for (int s = 0; s < 2; ++s)
+#pragma unroll
+                for (int b = 0; b < DB; ++b) {
+                    if (y == 0) dv[b] = mma(tile::cols(lds_g, 16 * s, 32 * b, lane), f[s], dv[b]);
+                    else dk[b] = mma(tile::cols(lds_q, 16 * s, 32 * b, lane), f[s], dk[b]);
+                }
+        }
+    }
+    if (r < length) {
+        if (r <= bad_query) {       // (a key that such a query sees: its gradients are not finite)
+#pragma unroll
+            for (int b = 0; b < DB; ++b) {
+                dk[b] += __builtin_nanf("");
+                dv[b] += __builtin_nanf("");
+            }
+        }
+        store_row<T>((T *)(p.d_k.p + (at + r) * p.d_k.ts + kvh * p.d_k.hs), dk, p.scale, d, lane);
+        store_row<T>((T *)(p.d_v.p + (at + r) * p.d_v.ts + kvh * p.d_v.hs), dv, 1.f, d, lane);
+    }
+}
+
 }  // namespace seq

@@ -10,12 +10,19 @@ SEQ_API int taco_attention_backward(const taco_attention_args *a, void *stream) 
         typedef decltype(type) T;
         constexpr int DP = decltype(dp)::value;
         const dim3 grid((unsigned)(p.n_tiles * p.heads)), grid_kv((unsigned)(p.n_tiles * p.kv_heads));
+        const hipStream_t s = (hipStream_t)stream;
+        if constexpr (short_gradients<T, DP>) {
+            if (a->whole) {
+                attention_short_grad_kernel<T, DP><<<grid_kv, 64, 0, s>>>(p);
+                return launched("taco_attention_backward");
+            }
+        }
         if (a->tile_rows == 32) {
-            attention_dq_kernel<T, DP, 1><<<grid, 64, 0, (hipStream_t)stream>>>(p);
-            attention_dkv_kernel<T, DP, 1><<<grid_kv, 64, 0, (hipStream_t)stream>>>(p);
+            attention_dq_kernel<T, DP, 1><<<grid, 64, 0, s>>>(p);
+            attention_dkv_kernel<T, DP, 1><<<grid_kv, 64, 0, s>>>(p);
         } else {
-            attention_dq_kernel<T, DP, 4><<<grid, 256, 0, (hipStream_t)stream>>>(p);
-            attention_dkv_kernel<T, DP, 4><<<grid_kv, 256, 0, (hipStream_t)stream>>>(p);
+            attention_dq_kernel<T, DP, 4><<<grid, 256, 0, s>>>(p);
+            attention_dkv_kernel<T, DP, 4><<<grid_kv, 256, 0, s>>>(p);
         }
         return launched("taco_attention_backward");
     });

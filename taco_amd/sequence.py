@@ -40,7 +40,7 @@ class Tensor(C.Structure):
 class AttentionArgs(C.Structure):
     """struct taco_attention_args"""
     _fields_ = [("q", Tensor), ("k", Tensor), ("v", Tensor), ("o", Tensor), ("lse", C.c_void_p), ("tiles", C.c_void_p), ("key_tiles", C.c_void_p),
-                ("n_tiles", C.c_int32), ("tile_rows", C.c_int32), ("heads", C.c_int32), ("kv_heads", C.c_int32), ("dim", C.c_int32), ("dtype", C.c_int32),
+                ("n_tiles", C.c_int32), ("tile_rows", C.c_int32), ("whole", C.c_int32), ("heads", C.c_int32), ("kv_heads", C.c_int32), ("dim", C.c_int32), ("dtype", C.c_int32),
                 ("causal", C.c_int32), ("scale", C.c_float), ("d_o", Tensor), ("d_q", Tensor), ("d_k", Tensor), ("d_v", Tensor), ("delta", C.c_void_p)]
 
 
@@ -218,23 +218,27 @@ class Packed:
         return got[0]
 
     def _tiles(self, heads):
-        """[(tile rows, tiles, key tiles, count)]: launches of 32- and of 128-row tiles.  A tile of 128 rows shares its loads between four wavefronts; sequences
-        of at most 64 tokens would leave half of it idle, and where all tiles together do not fill the CUs, smaller ones spread the work."""
+        """[(tile rows, tiles, key tiles, count, how many of them at the end are whole sequences)].  A tile of 128 rows shares its loads between four wavefronts;
+        sequences of at most 64 tokens would leave half of it idle, and where all tiles together do not fill the CUs, smaller ones spread the work.  Sequences
+        of at most 32 tokens are a tile each."""
         wide = self._wide_tiles * heads >= 256
         key = "wide tiles" if wide else "tiles"
 
+        def tiles(rows, which):
+            which = np.flatnonzero(which)
+            n = -(-self.lengths[which] // rows)
+            of = np.repeat(which, n)
+            first = (np.arange(len(of)) - np.repeat(np.cumsum(n) - n, n)) * rows
+            t = np.stack([self.starts[of], self.lengths[of], first, np.zeros_like(first)], 1).astype(np.int32)
+            return t[np.argsort(-np.minimum(first + rows, self.lengths[of]), kind="stable")], t[np.argsort(first - self.lengths[of], kind="stable")]
+
         def make():
-            out, big = [], (self.lengths > 64) & wide
-            for rows, which in ((128, np.flatnonzero(big)), (32, np.flatnonzero(~big & (self.lengths > 0)))):
-                n = -(-self.lengths[which] // rows)
-                of = np.repeat(which, n)
-                first = (np.arange(len(of)) - np.repeat(np.cumsum(n) - n, n)) * rows
-                if len(of):
-                    t = np.stack([self.starts[of], self.lengths[of], first, np.zeros_like(first)], 1).astype(np.int32)
-                    out += [rows, t[np.argsort(-np.minimum(first + rows, self.lengths[of]), kind="stable")], t[np.argsort(first - self.lengths[of], kind="stable")], len(of)]
-            return out
+            big, short = (self.lengths > 64) & wide, self.lengths <= 32
+            large, some, whole = tiles(128, big), tiles(32, ~big & ~short), tiles(32, short & (self.lengths > 0))
+            small = [np.concatenate(x) for x in zip(some, whole)]
+            return (128, *large, len(large[0]), 0, 32, *small, len(small[0]), len(whole[0]))
         got = self._kept(key, make)
-        return [got[i:i + 4] for i in range(0, len(got), 4)]
+        return [got[i:i + 5] for i in (0, 5) if got[i + 3]]
 
     def _segments(self, work):
         """(segments, first segment of each sequence, count) for `work` = heads x products.  A workgroup fills a CU, so pieces of half a CU's share of all tokens
@@ -260,13 +264,24 @@ class Packed:
 
 def _attention_args(q, k, v, o, lse, seqs, causal, scale):
     heads, dim = q.shape[1], q.shape[2]
-    return AttentionArgs(_tensor(q), _tensor(k), _tensor(v), _tensor(o), lse.data_ptr(), None, None, 0, 0, heads, k.shape[1], dim, _DTYPES[q.dtype], 1 if causal else 0, scale)
+    return AttentionArgs(_tensor(q), _tensor(k), _tensor(v), _tensor(o), lse.data_ptr(), None, None, 0, 0, 0, heads, k.shape[1], dim, _DTYPES[q.dtype], 1 if causal else 0, scale)
 
 
-def _launch_tiles(f, a, seqs, device):
-    for rows, tiles, key_tiles, count in seqs._tiles(a.heads):
-        a.tiles, a.key_tiles, a.n_tiles, a.tile_rows = tiles.data_ptr(), key_tiles.data_ptr(), count, rows
-        _call(f, a, device)
+def _launch_tiles(a, seqs, device, backward):
+    lib = load()
+    for rows, tiles, key_tiles, count, whole in seqs._tiles(a.heads):
+        a.tile_rows, a.tiles, a.key_tiles, a.n_tiles = rows, tiles.data_ptr(), key_tiles.data_ptr(), count
+        if not backward:
+            _call(lib.taco_attention, a, device)
+            continue
+        a.n_tiles = count - whole           # (whole sequences have a launch of their own)
+        if a.n_tiles:
+            _call(lib.taco_attention_backward, a, device)
+        if whole:
+            skip = (count - whole) * C.sizeof(C.c_int32 * 4)
+            a.tiles, a.key_tiles, a.n_tiles, a.whole = a.tiles + skip, a.key_tiles + skip, whole, 1
+            _call(lib.taco_attention_backward, a, device)
+            a.whole = 0
 
 
 def _empty(shape, total, dtype, device):
@@ -283,7 +298,7 @@ def _attention_forward(q, k, v, seqs, causal, scale, out):
     o = _empty(q.shape, total, q.dtype, device) if out is None else out
     lse = _empty(q.shape[:2], total, torch.float32, device)
     if total:
-        _launch_tiles(load().taco_attention, _attention_args(q, k, v, o, lse, seqs, causal, scale), seqs, device)
+        _launch_tiles(_attention_args(q, k, v, o, lse, seqs, causal, scale), seqs, device, False)
     return q, k, v, o, lse
 
 
@@ -310,7 +325,7 @@ class _Attention(torch.autograd.Function):
             a = _attention_args(q, k, v, o, lse, seqs, causal, scale)
             delta = torch.empty(q.shape[:2], dtype=torch.float32, device=q.device)
             a.d_o, a.d_q, a.d_k, a.d_v, a.delta = _tensor(d_o), _tensor(dq), _tensor(dk), _tensor(dv), delta.data_ptr()
-            _launch_tiles(load().taco_attention_backward, a, seqs, q.device)
+            _launch_tiles(a, seqs, q.device, True)
         return dq, dk, dv, None, None, None
 
 

@@ -52,7 +52,7 @@ def tensor(p=1 << 20, ts=64, hs=32):
 
 
 def attention_args(**kw):
-    a = sequence.AttentionArgs(tensor(), tensor(), tensor(), tensor(), 1 << 20, 1 << 20, None, 1, 128, 2, 2, 32, 0, 1, 1.0, tensor(), tensor(), tensor(), tensor(), 1 << 20)
+    a = sequence.AttentionArgs(tensor(), tensor(), tensor(), tensor(), 1 << 20, 1 << 20, None, 1, 128, 0, 2, 2, 32, 0, 1, 1.0, tensor(), tensor(), tensor(), tensor(), 1 << 20)
     for k, v in kw.items():
         setattr(a, k, v)
     return a
@@ -84,7 +84,7 @@ BAD_TENSORS = [tensor(p=None), tensor(p=(1 << 20) + 8), tensor(ts=30), tensor(ts
 
 @pytest.mark.parametrize("name,make,bad", [
     ("taco_attention", attention_args, [dict(dim=12), dict(dim=0), dict(dim=136), dict(dtype=3), dict(heads=3), dict(kv_heads=0), dict(scale=0.0), dict(scale=float("nan")),
-                                        dict(scale=float("inf")), dict(tile_rows=64), dict(n_tiles=-1), dict(n_tiles=1 << 30, heads=4), dict(lse=None), dict(tiles=None)]
+                                        dict(scale=float("inf")), dict(tile_rows=64), dict(whole=1), dict(n_tiles=-1), dict(n_tiles=1 << 30, heads=4), dict(lse=None), dict(tiles=None)]
      + [{f: t} for f in "qkvo" for t in BAD_TENSORS]),
     ("taco_attention_backward", attention_args, [dict(delta=None)] + [{f: t} for f in ("d_o", "d_q", "d_k", "d_v") for t in BAD_TENSORS]),
     ("taco_attention_step", step_args, [dict(rows=-1), dict(num_pages=0), dict(page_size=0), dict(table_width=0), dict(table=None), dict(lengths=None), dict(k_pages=None),
@@ -217,15 +217,15 @@ def lists(monkeypatch, lens):
 def test_tiles_cover_every_token_once(monkeypatch, lens, heads):
     seqs = lists(monkeypatch, lens)
     seen = np.zeros(sum(lens), int)
-    for rows, tiles, key_tiles, count in seqs._tiles(heads):
-        assert rows in (32, 128) and tiles.shape == (count, 4) and tiles.dtype == np.int32
+    for rows, tiles, key_tiles, count, whole in seqs._tiles(heads):
+        assert rows in (32, 128) and (rows == 32 or not whole) and (tiles[count - whole:, 1] <= 32).all() and (key_tiles[count - whole:, 1] <= 32).all() and tiles.shape == (count, 4) and tiles.dtype == np.int32
         assert sorted(map(tuple, tiles)) == sorted(map(tuple, key_tiles))
         for start, length, first, _ in tiles:
             assert first % rows == 0 and 0 <= first < length and (start, length) in set(zip(seqs.starts, seqs.lengths))
             seen[start + first:start + min(first + rows, length)] += 1
-        last = np.minimum(tiles[:, 2] + rows, tiles[:, 1])
-        assert (np.diff(last) <= 0).all()                       # the longest first
-        assert (np.diff(key_tiles[:, 1] - key_tiles[:, 2]) <= 0).all()
+        for part in (slice(0, count - whole), slice(count - whole, count)):      # the longest first
+            assert (np.diff(np.minimum(tiles[part, 2] + rows, tiles[part, 1])) <= 0).all()
+            assert (np.diff(key_tiles[part, 1] - key_tiles[part, 2]) <= 0).all()
     assert (seen == 1).all()
 
 

@@ -65,7 +65,7 @@ def test_attention_in_tiles_of_128_rows(dtype, d):
     lens = [129, 64, 300, 1, 128]
     check_attention(60, 20, d, lens, dtype)
     seqs = S().Packed(lens, "cuda:0")
-    assert [x[0] for x in seqs._tiles(60)] == [128, 32]
+    assert [(x[0], x[3], x[4]) for x in seqs._tiles(60)] == [(128, 6, 0), (32, 3, 1)]
 
 
 @pytest.mark.parametrize("dtype", DTYPES)
