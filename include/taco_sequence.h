@@ -55,6 +55,9 @@ typedef struct taco_attention_args {
     /* backward only: */
     taco_seq_tensor d_o, d_q, d_k, d_v;
     float *delta;                       /* workspace [tokens][heads] */
+    int32_t parts;                      /* 128-row tiles: a key-value head's group of query heads in that many parts (a divisor of heads / kv_heads), each a
+                                           workgroup of its own; more than 1 needs the workspace [tokens][kv_heads][parts][2][dim padded to 32, 64 or 128] */
+    float *partial;
 } taco_attention_args;
 int taco_attention(const taco_attention_args *a, void *stream);
 /* Gradients by the formulas (P from lse; dS = P (dP - rowsum(d_o o))): two launches, the second reads `delta`, which the first writes; one launch where

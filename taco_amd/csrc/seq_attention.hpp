@@ -14,8 +14,9 @@ struct AttentionParams {
     View q, k, v, o, d_o, d_q, d_k, d_v;
     float *lse, *delta;
     const taco_seq_tile *tiles, *key_tiles;
-    int32_t n_tiles, heads, kv_heads, dim, causal;
+    int32_t n_tiles, heads, kv_heads, dim, causal, parts;
     float scale;
+    float *partial;          // [tokens][kv_heads][parts][2][DP]
 };
 
 // Workgroups go to the 8 XCDs in turn, each with an L2 of its own: with a multiple of 8 heads, neighbouring heads (one group's, which read the same keys and
@@ -29,7 +30,8 @@ __device__ __forceinline__ void locate(int block, int heads, int &tile, int &hea
 // Wavefronts per SIMD that the registers are cut for: as many as do not spill.  Nothing else hides the latency of loads and of the chain of products, least
 // of all where a sequence is one tile.
 template <typename T, int DP, int NW> constexpr int waves_forward = sizeof(T) == 4 ? (DP == 32 ? 2 : 1) : DP == 32 ? 4 : DP == 64 || NW == 4 ? 2 : 1;
-template <typename T, int DP> constexpr int waves_backward = sizeof(T) == 4 ? (DP == 32 ? 2 : 1) : DP <= 64 ? 2 : 1;
+template <typename T, int DP> constexpr int waves_dq = sizeof(T) == 4 ? (DP == 32 ? 2 : 1) : 2;
+template <typename T, int DP> constexpr int waves_dkv = sizeof(T) == 4 ? (DP == 32 ? 2 : 1) : DP <= 64 ? 2 : 1;
 // The next tiles travel in registers while these are used, except where that would spill: float32 rows of 128 hold half the registers as operands already.
 template <typename T, int DP> constexpr bool ahead = !(sizeof(T) == 4 && DP == 128);
 
@@ -210,7 +212,7 @@ __global__ __launch_bounds__(64 * NW, (waves_forward<T, DP, NW>)) void attention
 // A query that sees few keys has gradients that are small differences of dP and delta, and o as it was rounded would set their error.  Where all its keys
 // lie in one tile, delta is the sum of P dP over that tile instead, in float32.
 template <typename T, int DP, int NW>
-__global__ __launch_bounds__(64 * NW, (waves_backward<T, DP>)) void attention_dq_kernel(AttentionParams p) {
+__global__ __launch_bounds__(64 * NW, (waves_dq<T, DP>)) void attention_dq_kernel(AttentionParams p) {
     typedef Tile<T, DP> tile;
     constexpr int BM = 32 * NW, BN = NW == 1 ? 32 : 64, NB = BN / 32, NS = DP / 16, DB = DP / 32, NT = 64 * NW;
     __shared__ __attribute__((aligned(16))) char lds_k[BN * tile::ROW], lds_v[BN * tile::ROW];
@@ -259,16 +261,8 @@ __global__ __launch_bounds__(64 * NW, (waves_backward<T, DP>)) void attention_dq
     auto weights = [&](int n, f32x16 &pr, f32x16 &dp) {
         f32x16 x[2];
         clear(x);
-#pragma unroll
-        for (int y = 0; y < NS; ++y) {
-            x[0] = mma(tile::rows(lds_k, 32 * n, y, lane), qf[y], x[0]);
-            in_order<T, DP>();
-        }
-#pragma unroll
-        for (int y = 0; y < NS; ++y) {
-            x[1] = mma(tile::rows(lds_v, 32 * n, y, lane), gf[y], x[1]);
-            in_order<T, DP>();
-        }
+        mma_rows<T>([&](int y) { return tile::rows(lds_k, 32 * n, y, lane); }, qf, x[0]);
+        mma_rows<T>([&](int y) { return tile::rows(lds_v, 32 * n, y, lane); }, gf, x[1]);
 #pragma unroll
         for (int i = 0; i < 16; ++i) pr[i] = exp2_(x[0][i] * c - mu);
         dp = x[1];
@@ -295,30 +289,23 @@ __global__ __launch_bounds__(64 * NW, (waves_backward<T, DP>)) void attention_dq
         if (ahead<T, DP> && kt > 0) fetch(kt - 1);
         const int k0 = kt * BN;
         if (!(p.causal && k0 > first + 31)) {      // (else: all of the tile is hidden from the wavefront)
-            f32x16 pr[NB], ds[NB];
-#pragma unroll
-            for (int n = 0; n < NB; ++n) {
-                weights(n, pr[n], ds[n]);
-#pragma unroll
-                for (int i = 0; i < 16; ++i) {
-                    const bool seen = k0 + 32 * n + row_of(i, h) <= limit;
-                    pr[n][i] = seen ? pr[n][i] : 0.f;
-                    ds[n][i] = seen ? ds[n][i] : 0.f;
-                }
-            }
+            f32x16 pr, ds;
             if (k0 == 0) {
                 float x = 0.f;
+#pragma unroll 1
+                for (int n = 0; n < NB; ++n) {
+                    weights(n, pr, ds);
 #pragma unroll
-                for (int n = 0; n < NB; ++n)
-#pragma unroll
-                    for (int i = 0; i < 16; ++i) x += pr[n][i] * ds[n][i];
+                    for (int i = 0; i < 16; ++i) x += k0 + 32 * n + row_of(i, h) <= limit ? pr[i] * ds[i] : 0.f;
+                }
                 delta = limit < BN ? x + other_half(x) : delta;
             }
-#pragma unroll
+#pragma unroll 1
             for (int n = 0; n < NB; ++n) {
+                weights(n, pr, ds);
 #pragma unroll
-                for (int i = 0; i < 16; ++i) ds[n][i] = k0 + 32 * n + row_of(i, h) <= limit ? pr[n][i] * (ds[n][i] - delta) : 0.f;
-                add_columns<T, DP>(lds_k, 32 * n, ds[n], dq, lane);
+                for (int i = 0; i < 16; ++i) ds[i] = k0 + 32 * n + row_of(i, h) <= limit ? pr[i] * (ds[i] - delta) : 0.f;
+                add_columns<T, DP>(lds_k, 32 * n, ds, dq, lane);
             }
             if (k0 + seen_bad <= limit && seen_bad < BN) {      // (a key that is not finite: its weight is not either)
 #pragma unroll
@@ -355,17 +342,21 @@ __global__ __launch_bounds__(64 * NW, (waves_backward<T, DP>)) void attention_dq
 // Backward, second launch: dK and dV.  A wavefront owns 32 keys, whose K and V rows stay in registers as operands; Q and dO tiles of BQ queries pass through LDS,
 // for every query head of the group in turn, so the gradients of a shared head are sums in registers.  S = Q K^T and dP = dO V^T have the keys in
 // the lanes; P and dS are the operands of dV^T = dO^T P and dK^T = Q^T dS as they stand.
+// Where the longest sequence's first keys would outlast everything else (all queries of all heads of the group behind one another), the group's heads are
+// shared out to `parts` workgroups, whose float32 sums a third launch adds up, always in the same order.
 template <typename T, int DP, int NW>
-__global__ __launch_bounds__(64 * NW, (waves_backward<T, DP>)) void attention_dkv_kernel(AttentionParams p) {
+__global__ __launch_bounds__(64 * NW, (waves_dkv<T, DP>)) void attention_dkv_kernel(AttentionParams p) {
     typedef Tile<T, DP> tile;
     constexpr int BK = 32 * NW, BQ = NW == 1 ? 32 : 64, NB = BQ / 32, NS = DP / 16, DB = DP / 32, NT = 64 * NW;
     __shared__ __attribute__((aligned(16))) char lds_q[BQ * tile::ROW], lds_g[BQ * tile::ROW];
     __shared__ __attribute__((aligned(16))) float lds_mu[BQ], lds_delta[BQ];
     __shared__ int nonfinite;       // the last query of the tile with something not finite in its row or its gradient's
     int ti, kvh;
-    locate(blockIdx.x, p.kv_heads, ti, kvh);
+    locate(blockIdx.x, p.kv_heads * p.parts, ti, kvh);
+    const int part = kvh % p.parts;
+    kvh /= p.parts;
     const taco_seq_tile w = p.key_tiles[ti];
-    const int t = threadIdx.x, lane = t & 63, wave = __builtin_amdgcn_readfirstlane(t >> 6), h = lane >> 5, d = p.dim, G = p.heads / p.kv_heads;
+    const int t = threadIdx.x, lane = t & 63, wave = __builtin_amdgcn_readfirstlane(t >> 6), h = lane >> 5, d = p.dim, G = p.heads / p.kv_heads / p.parts, head0 = (kvh * p.parts + part) * G;
     const int first = w.first + 32 * wave, key = first + (lane & 31);
     const uint32_t rb = d * sizeof(T);
     const float c = p.scale * LOG2E;
@@ -411,16 +402,8 @@ __global__ __launch_bounds__(64 * NW, (waves_backward<T, DP>)) void attention_dk
     // P and dS of 32 queries
     auto weights = [&](int n, f32x16 (&x)[2]) {
         clear(x);
-#pragma unroll
-        for (int y = 0; y < NS; ++y) {
-            x[0] = mma(tile::rows(lds_q, 32 * n, y, lane), kf[y], x[0]);
-            in_order<T, DP>();
-        }
-#pragma unroll
-        for (int y = 0; y < NS; ++y) {
-            x[1] = mma(tile::rows(lds_g, 32 * n, y, lane), vf[y], x[1]);
-            in_order<T, DP>();
-        }
+        mma_rows<T>([&](int y) { return tile::rows(lds_q, 32 * n, y, lane); }, kf, x[0]);
+        mma_rows<T>([&](int y) { return tile::rows(lds_g, 32 * n, y, lane); }, vf, x[1]);
 #pragma unroll
         for (int i = 0; i < 16; i += 4) {
             f32x4 mu = *(const f32x4 *)(lds_mu + 32 * n + row_of(i, h)), de = *(const f32x4 *)(lds_delta + 32 * n + row_of(i, h));
@@ -431,14 +414,14 @@ __global__ __launch_bounds__(64 * NW, (waves_backward<T, DP>)) void attention_dk
             }
         }
     };
-    if (ahead<T, DP>) fetch(kvh * G, qt0);
+    if (ahead<T, DP>) fetch(head0, qt0);
     if (t == 0) nonfinite = -1;
-    for (int head = kvh * G; head < (kvh + 1) * G; ++head) {
+    for (int head = head0; head < head0 + G; ++head) {
         int qt = qt0;
         auto next = [&]() {
             if (!ahead<T, DP>) return;
             if (qt + 1 < qt1) fetch(head, qt + 1);
-            else if (head + 1 < (kvh + 1) * G) fetch(head + 1, qt0);
+            else if (head + 1 < head0 + G) fetch(head + 1, qt0);
         };
         for (; qt < whole; ++qt) {
             __syncthreads();
@@ -496,9 +479,36 @@ __global__ __launch_bounds__(64 * NW, (waves_backward<T, DP>)) void attention_dk
             }
         }
     }
-    if (key < w.length) {
+    if (NW == 4 && p.parts > 1) {
+        float *to = p.partial + (((int64_t)(w.start + key) * p.kv_heads + kvh) * p.parts + part) * 2 * DP;
+        if (key < w.length) {
+            store_row<float>(to, dk, 1.f, DP, lane);
+            store_row<float>(to + DP, dv, 1.f, DP, lane);
+        }
+    } else if (key < w.length) {
         store_row<T>((T *)(p.d_k.p + (int64_t)(w.start + key) * p.d_k.ts + kvh * p.d_k.hs), dk, p.scale, d, lane);
         store_row<T>((T *)(p.d_v.p + (int64_t)(w.start + key) * p.d_v.ts + kvh * p.d_v.hs), dv, 1.f, d, lane);
+    }
+}
+
+template <typename T, int DP> __global__ __launch_bounds__(256) void attention_sum_kernel(AttentionParams p) {
+    int ti, kvh;
+    locate(blockIdx.x, p.kv_heads, ti, kvh);
+    const taco_seq_tile w = p.key_tiles[ti];
+    const int rows = min(128, w.length - w.first);
+    for (int e = threadIdx.x; e < rows * (DP / 4); e += 256) {
+        const int64_t token = w.start + w.first + e / (DP / 4);
+        const int x = e % (DP / 4) * 4;
+        const float *from = p.partial + (token * p.kv_heads + kvh) * p.parts * 2 * DP + x;
+        f32x4 dk{0, 0, 0, 0}, dv{0, 0, 0, 0};
+        for (int i = 0; i < p.parts; ++i) {
+            dk += *(const f32x4 *)(from + i * 2 * DP);
+            dv += *(const f32x4 *)(from + i * 2 * DP + DP);
+        }
+        if (x < p.dim) {
+            store4((T *)(p.d_k.p + token * p.d_k.ts + kvh * p.d_k.hs) + x, dk[0] * p.scale, dk[1] * p.scale, dk[2] * p.scale, dk[3] * p.scale);
+            store4((T *)(p.d_v.p + token * p.d_v.ts + kvh * p.d_v.hs) + x, dv[0], dv[1], dv[2], dv[3]);
+        }
     }
 }
 

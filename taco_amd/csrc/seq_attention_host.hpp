@@ -23,6 +23,14 @@ inline int attention_params(const taco_attention_args *a, bool backward, Attenti
     }
     SEQ_NEED(a->lse && a->tiles, "lse or tiles: null");
     SEQ_NEED(!backward || a->delta, "delta: null");
+    p.parts = 1;
+    if (backward && a->tile_rows == 128) {
+        SEQ_NEED(a->parts >= 1 && (a->heads / a->kv_heads) % a->parts == 0, "%d parts of a group of %d query heads", a->parts, a->heads / a->kv_heads);
+        SEQ_NEED(a->parts == 1 || (a->partial && (uintptr_t)a->partial % 16 == 0), "partial: null or not 16-byte aligned");
+        SEQ_NEED((int64_t)a->n_tiles * a->kv_heads * a->parts < (int64_t)1 << 31, "%d tiles of %d heads in %d parts: fewer than 2^31 in all", a->n_tiles, a->kv_heads, a->parts);
+        p.parts = a->parts;
+        p.partial = a->partial;
+    }
     p.lse = a->lse;
     p.delta = a->delta;
     p.tiles = a->tiles;

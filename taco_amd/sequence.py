@@ -41,7 +41,8 @@ class AttentionArgs(C.Structure):
     """struct taco_attention_args"""
     _fields_ = [("q", Tensor), ("k", Tensor), ("v", Tensor), ("o", Tensor), ("lse", C.c_void_p), ("tiles", C.c_void_p), ("key_tiles", C.c_void_p),
                 ("n_tiles", C.c_int32), ("tile_rows", C.c_int32), ("whole", C.c_int32), ("heads", C.c_int32), ("kv_heads", C.c_int32), ("dim", C.c_int32), ("dtype", C.c_int32),
-                ("causal", C.c_int32), ("scale", C.c_float), ("d_o", Tensor), ("d_q", Tensor), ("d_k", Tensor), ("d_v", Tensor), ("delta", C.c_void_p)]
+                ("causal", C.c_int32), ("scale", C.c_float), ("d_o", Tensor), ("d_q", Tensor), ("d_k", Tensor), ("d_v", Tensor), ("delta", C.c_void_p),
+                ("parts", C.c_int32), ("partial", C.c_void_p)]
 
 
 class AttentionStepArgs(C.Structure):
@@ -199,6 +200,7 @@ class Packed:
             raise ValueError(f"{self.total} tokens: fewer than 2^31 - 4096 are supported")
         self._lists = {}
         self._wide_tiles = int((-(-n[n > 64] // 128)).sum())
+        self._longest, self._pairs = int(n.max(initial=0)), float((n[n > 64].astype(np.float64) ** 2).sum())
 
     def __len__(self):
         return len(self.lengths)
@@ -239,6 +241,15 @@ class Packed:
             return (128, *large, len(large[0]), 0, 32, *small, len(small[0]), len(whole[0]))
         got = self._kept(key, make)
         return [got[i:i + 5] for i in (0, 5) if got[i + 3]]
+
+    def _parts(self, heads, group, causal):
+        """Into how many parts the backward's second launch shares out a group's query heads: few enough that their partial sums' way through memory stays small, but
+        so many that the longest sequence's first tile of keys, which sees all its queries, takes no longer than a CU's share of everything."""
+        share = self._pairs * (0.5 if causal else 1.0) * heads / 128 / 256
+        for parts in range(1, group + 1):
+            if group % parts == 0 and self._longest * (group // parts) <= share:
+                return parts
+        return group
 
     def _segments(self, work):
         """(segments, first segment of each sequence, count) for `work` = heads x products.  A workgroup fills a CU, so pieces of half a CU's share of all tokens
@@ -325,6 +336,11 @@ class _Attention(torch.autograd.Function):
             a = _attention_args(q, k, v, o, lse, seqs, causal, scale)
             delta = torch.empty(q.shape[:2], dtype=torch.float32, device=q.device)
             a.d_o, a.d_q, a.d_k, a.d_v, a.delta = _tensor(d_o), _tensor(dq), _tensor(dk), _tensor(dv), delta.data_ptr()
+            H, Hk, d = q.shape[1], k.shape[1], q.shape[2]
+            a.parts = 1 if H == Hk else seqs._parts(H, H // Hk, causal)
+            if a.parts > 1:
+                partial = torch.empty((seqs.total, Hk, a.parts, 2, 32 if d <= 32 else 64 if d <= 64 else 128), dtype=torch.float32, device=q.device)
+                a.partial = partial.data_ptr()
             _launch_tiles(a, seqs, q.device, True)
         return dq, dk, dv, None, None, None
 

@@ -52,7 +52,7 @@ def tensor(p=1 << 20, ts=64, hs=32):
 
 
 def attention_args(**kw):
-    a = sequence.AttentionArgs(tensor(), tensor(), tensor(), tensor(), 1 << 20, 1 << 20, None, 1, 128, 0, 2, 2, 32, 0, 1, 1.0, tensor(), tensor(), tensor(), tensor(), 1 << 20)
+    a = sequence.AttentionArgs(tensor(), tensor(), tensor(), tensor(), 1 << 20, 1 << 20, None, 1, 128, 0, 2, 2, 32, 0, 1, 1.0, tensor(), tensor(), tensor(), tensor(), 1 << 20, 1, None)
     for k, v in kw.items():
         setattr(a, k, v)
     return a
@@ -86,7 +86,7 @@ BAD_TENSORS = [tensor(p=None), tensor(p=(1 << 20) + 8), tensor(ts=30), tensor(ts
     ("taco_attention", attention_args, [dict(dim=12), dict(dim=0), dict(dim=136), dict(dtype=3), dict(heads=3), dict(kv_heads=0), dict(scale=0.0), dict(scale=float("nan")),
                                         dict(scale=float("inf")), dict(tile_rows=64), dict(whole=1), dict(n_tiles=-1), dict(n_tiles=1 << 30, heads=4), dict(lse=None), dict(tiles=None)]
      + [{f: t} for f in "qkvo" for t in BAD_TENSORS]),
-    ("taco_attention_backward", attention_args, [dict(delta=None)] + [{f: t} for f in ("d_o", "d_q", "d_k", "d_v") for t in BAD_TENSORS]),
+    ("taco_attention_backward", attention_args, [dict(delta=None), dict(parts=0), dict(parts=3), dict(parts=2, kv_heads=1)] + [{f: t} for f in ("d_o", "d_q", "d_k", "d_v") for t in BAD_TENSORS]),
     ("taco_attention_step", step_args, [dict(rows=-1), dict(num_pages=0), dict(page_size=0), dict(table_width=0), dict(table=None), dict(lengths=None), dict(k_pages=None),
                                         dict(v_pages=(1 << 20) + 4), dict(k_page_stride=1022), dict(v_token_stride=-64), dict(scale=-1.0), dict(rows=1 << 30, heads=2),
                                         dict(k_new=tensor(p=None)), dict(v_new=tensor(p=None)), dict(q=tensor(hs=16))] + [{f: t} for f in ("q", "o") for t in BAD_TENSORS]),

@@ -69,6 +69,15 @@ def test_attention_in_tiles_of_128_rows(dtype, d):
 
 
 @pytest.mark.parametrize("dtype", DTYPES)
+def test_attention_group_in_parts(dtype):
+    """one long sequence, few key-value heads: the group's heads are shared out, and their sums joined"""
+    lens = [700, 129]
+    seqs = S().Packed(lens, "cuda:0")
+    assert seqs._parts(64, 32, True) > 1 and seqs._tiles(64)[0][0] == 128
+    check_attention(64, 2, 24, lens, dtype)
+
+
+@pytest.mark.parametrize("dtype", DTYPES)
 def test_attention_not_causal(dtype):
     check_attention(4, 2, 48, [1, 33, 64, 70, 130], dtype, causal=False)
     check_attention(64, 64, 32, [129, 260, 100], dtype, causal=False, train=False)
@@ -81,11 +90,11 @@ def test_attention_scale_and_large_scores():
 
 
 @pytest.mark.parametrize("dtype", DTYPES)
-@pytest.mark.parametrize("H", [2, 130])
+@pytest.mark.parametrize("H,lens,bad", [(2, [70, 150, 33], 41), (130, [70, 150, 33], 41), (2, [9, 30, 32], 11)])
 @pytest.mark.parametrize("poison", [float("nan"), float("inf"), -float("inf")])
-def test_hidden_tokens_have_no_influence(dtype, H, poison):
-    """a token that diverges at step 41 of a sequence: the steps before it, and the other sequences, get the bits they get without it, forward and backward"""
-    lens, d, bad = [70, 150, 33], 64, 41
+def test_hidden_tokens_have_no_influence(dtype, H, lens, bad, poison):
+    """a token that diverges at one step of a sequence: the steps before it, and the other sequences, get the bits they get without it, forward and backward"""
+    d = 64
     T = sum(lens)
     at = lens[0] + bad
     q, k, v, g = (randn(T, H, d, dtype=dtype, seed=i) for i in range(4))
