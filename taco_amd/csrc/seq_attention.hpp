@@ -30,7 +30,7 @@ __device__ __forceinline__ void locate(int block, int heads, int &tile, int &hea
 // Wavefronts per SIMD that the registers are cut for: as many as do not spill.  Nothing else hides the latency of loads and of the chain of products, least
 // of all where a sequence is one tile.
 template <typename T, int DP, int NW> constexpr int waves_forward = sizeof(T) == 4 ? (DP == 32 ? 2 : 1) : DP == 32 ? 4 : DP == 64 || NW == 4 ? 2 : 1;
-template <typename T, int DP> constexpr int waves_dq = sizeof(T) == 4 ? (DP == 32 ? 2 : 1) : 2;
+template <typename T, int DP, int NW> constexpr int waves_dq = sizeof(T) == 4 ? (DP == 32 ? 2 : 1) : DP <= 64 || NW == 4 ? 2 : 1;
 template <typename T, int DP> constexpr int waves_dkv = sizeof(T) == 4 ? (DP == 32 ? 2 : 1) : DP <= 64 ? 2 : 1;
 // The next tiles travel in registers while these are used, except where that would spill: float32 rows of 128 hold half the registers as operands already.
 template <typename T, int DP> constexpr bool ahead = !(sizeof(T) == 4 && DP == 128);
@@ -92,7 +92,7 @@ __global__ __launch_bounds__(64 * NW, (waves_forward<T, DP, NW>)) void attention
     const char *kp = p.k.p + (int64_t)w.start * p.k.ts + kvh * p.k.hs, *vp = p.v.p + (int64_t)w.start * p.v.ts + kvh * p.v.hs;
     Staged<T, DP, BN, NT> sk, sv;
     auto fetch = [&](int kt) {
-        int n = min(BN, w.length - kt * BN);
+        const int n = min(BN, w.length - kt * BN);
         sk.load(rows_of(kp + (int64_t)kt * BN * p.k.ts, n, p.k.ts, rb), p.k.ts, d, t);
         sv.load(rows_of(vp + (int64_t)kt * BN * p.v.ts, n, p.v.ts, rb), p.v.ts, d, t);
     };
@@ -212,7 +212,7 @@ __global__ __launch_bounds__(64 * NW, (waves_forward<T, DP, NW>)) void attention
 // A query that sees few keys has gradients that are small differences of dP and delta, and o as it was rounded would set their error.  Where all its keys
 // lie in one tile, delta is the sum of P dP over that tile instead, in float32.
 template <typename T, int DP, int NW>
-__global__ __launch_bounds__(64 * NW, (waves_dq<T, DP>)) void attention_dq_kernel(AttentionParams p) {
+__global__ __launch_bounds__(64 * NW, (waves_dq<T, DP, NW>)) void attention_dq_kernel(AttentionParams p) {
     typedef Tile<T, DP> tile;
     constexpr int BM = 32 * NW, BN = NW == 1 ? 32 : 64, NB = BN / 32, NS = DP / 16, DB = DP / 32, NT = 64 * NW;
     __shared__ __attribute__((aligned(16))) char lds_k[BN * tile::ROW], lds_v[BN * tile::ROW];
@@ -248,9 +248,9 @@ __global__ __launch_bounds__(64 * NW, (waves_dq<T, DP>)) void attention_dq_kerne
     const char *kp = p.k.p + (int64_t)w.start * p.k.ts + kvh * p.k.hs, *vp = p.v.p + (int64_t)w.start * p.v.ts + kvh * p.v.hs;
     Staged<T, DP, BN, NT> sk, sv;
     auto fetch = [&](int kt) {
-        int n = min(BN, w.length - kt * BN);
-        sk.load(rows_of(kp + (int64_t)kt * BN * p.k.ts, n, p.k.ts, rb), p.k.ts, d, t);
-        sv.load(rows_of(vp + (int64_t)kt * BN * p.v.ts, n, p.v.ts, rb), p.v.ts, d, t);
+        const int n = min(BN, w.length - kt * BN), t_ = afresh(t);
+        sk.load(rows_of(kp + (int64_t)kt * BN * p.k.ts, n, p.k.ts, rb), p.k.ts, d, t_);
+        sv.load(rows_of(vp + (int64_t)kt * BN * p.v.ts, n, p.v.ts, rb), p.v.ts, d, t_);
     };
 
     f32x16 dq[DB];
@@ -486,6 +486,176 @@ __global__ __launch_bounds__(64 * NW, (waves_dkv<T, DP>)) void attention_dkv_ker
             store_row<float>(to + DP, dv, 1.f, DP, lane);
         }
     } else if (key < w.length) {
+        store_row<T>((T *)(p.d_k.p + (int64_t)(w.start + key) * p.d_k.ts + kvh * p.d_k.hs), dk, p.scale, d, lane);
+        store_row<T>((T *)(p.d_v.p + (int64_t)(w.start + key) * p.d_v.ts + kvh * p.d_v.hs), dv, 1.f, d, lane);
+    }
+}
+
+// The same for 128 keys of 16 bits and rows of 128, where the operands and sums of 32 keys leave room for one wavefront on a SIMD only, and nothing to hide its
+// waits behind.  K and V stay in LDS instead, and two wavefronts own the same 32 keys: one takes the first 32 queries of each tile, one the others; their
+// sums meet in LDS at the end.
+template <typename T, int DP> constexpr bool keys_in_lds = sizeof(T) == 2 && DP == 128;
+template <typename T, int DP>
+__global__ __launch_bounds__(512, 2) void attention_dkv_pair_kernel(AttentionParams p) {
+    typedef Tile<T, DP> tile;
+    constexpr int BK = 128, BQ = 64, NS = DP / 16, DB = DP / 32, NT = 512, KT = BK * tile::ROW, QT = BQ * tile::ROW;
+    __shared__ __attribute__((aligned(16))) char lds[2 * KT + 2 * QT];
+    __shared__ __attribute__((aligned(16))) float lds_mu[BQ], lds_delta[BQ];
+    __shared__ int nonfinite;       // the last query of the tile with something not finite in its row or its gradient's
+    char *const lds_k = lds, *const lds_v = lds + KT, *const lds_q = lds + 2 * KT, *const lds_g = lds + 2 * KT + QT;
+    static_assert(4 * DB * 16 * 64 * sizeof(float) <= sizeof(lds), "the sums of four wavefronts");
+    int ti, kvh;
+    locate(blockIdx.x, p.kv_heads * p.parts, ti, kvh);
+    const int part = kvh % p.parts;
+    kvh /= p.parts;
+    const taco_seq_tile w = p.key_tiles[ti];
+    const int t = threadIdx.x, lane = t & 63, wave = __builtin_amdgcn_readfirstlane(t >> 6), keys = 32 * (wave & 3), half = wave >> 2, h = lane >> 5, d = p.dim;
+    const int G = p.heads / p.kv_heads / p.parts, head0 = (kvh * p.parts + part) * G, first = w.first + keys, key = first + (lane & 31);
+    const uint32_t rb = d * sizeof(T);
+    const float c = p.scale * LOG2E;
+    {
+        const int64_t at = w.start + w.first;
+        const int n = min(BK, w.length - w.first);
+        Staged<T, DP, BK, NT> s;
+        s.load(rows_of(p.k.p + at * p.k.ts + kvh * p.k.hs, n, p.k.ts, rb), p.k.ts, d, t);
+        s.put(lds_k, t);
+        s.load(rows_of(p.v.p + at * p.v.ts + kvh * p.v.hs, n, p.v.ts, rb), p.v.ts, d, t);
+        s.put(lds_v, t);
+    }
+    const int qt0 = p.causal ? w.first / BQ : 0, qt1 = (w.length - 1) / BQ + 1;
+    const int whole = p.causal ? min(qt1, (w.first + BK) / BQ) : 0;      // tiles from here on hide no key of the workgroup
+    Staged<T, DP, BQ, NT> sq, sg;
+    float mu_r = 0.f, delta_r = 0.f;
+    auto fetch = [&](int head, int qt) {
+        const int q0 = qt * BQ, n = min(BQ, w.length - q0), t_ = afresh(t);
+        const int64_t at = w.start + q0;
+        sq.load(rows_of(p.q.p + at * p.q.ts + head * p.q.hs, n, p.q.ts, rb), p.q.ts, d, t_);
+        sg.load(rows_of(p.d_o.p + at * p.d_o.ts + head * p.d_o.hs, n, p.d_o.ts, rb), p.d_o.ts, d, t_);
+        if (t < BQ) {
+            float lse = t < n ? p.lse[(at + t) * p.heads + head] : -__builtin_inff();
+            delta_r = t < n ? p.delta[(at + t) * p.heads + head] : 0.f;
+            mu_r = lse == -__builtin_inff() ? __builtin_inff() : lse * LOG2E;
+        }
+    };
+    auto put = [&]() {
+        sq.put(lds_q, t);
+        sg.put(lds_g, t);
+        if (t < BQ) {
+            lds_mu[t] = mu_r;
+            lds_delta[t] = delta_r;
+        }
+    };
+    f32x16 dk[DB], dv[DB];
+    clear(dk);
+    clear(dv);
+    // P and dS of this wavefront's 32 queries
+    auto weights = [&](f32x16 (&x)[2]) {
+        clear(x);
+#pragma unroll
+        for (int z = 0; z < 2; ++z)
+#pragma unroll
+            for (int y0 = 0; y0 < NS; y0 += 4) {
+                frag<T> a[4], b[4];
+#pragma unroll
+                for (int y = 0; y < 4; ++y) {
+                    a[y] = tile::rows(z ? lds_g : lds_q, 32 * half, y0 + y, lane);
+                    b[y] = tile::rows(z ? lds_v : lds_k, keys, y0 + y, lane);
+                }
+                __builtin_amdgcn_sched_barrier(0);
+#pragma unroll
+                for (int y = 0; y < 4; ++y) x[z] = mma(a[y], b[y], x[z]);
+            }
+#pragma unroll
+        for (int i = 0; i < 16; i += 4) {
+            f32x4 mu = *(const f32x4 *)(lds_mu + 32 * half + row_of(i, h)), de = *(const f32x4 *)(lds_delta + 32 * half + row_of(i, h));
+#pragma unroll
+            for (int j = 0; j < 4; ++j) {
+                x[0][i + j] = exp2_(x[0][i + j] * c - mu[j]);
+                x[1][i + j] = x[0][i + j] * (x[1][i + j] - de[j]);
+            }
+        }
+    };
+    fetch(head0, qt0);
+    if (t == 0) nonfinite = -1;
+    for (int head = head0; head < head0 + G; ++head) {
+        int qt = qt0;
+        auto next = [&]() {
+            if (qt + 1 < qt1) fetch(head, qt + 1);
+            else if (head + 1 < head0 + G) fetch(head + 1, qt0);
+        };
+        for (; qt < whole; ++qt) {
+            __syncthreads();
+            if (__any(sq.any_nonfinite() || sg.any_nonfinite())) {
+                int r = -1;
+#pragma unroll
+                for (int i = 0; i < Staged<T, DP, BQ, NT>::N; ++i)
+                    if (sq.chunk_nonfinite(i) || sg.chunk_nonfinite(i)) r = (i * NT + t) / tile::NC;
+                sq.nonfinite_to_zero();
+                sg.nonfinite_to_zero();
+                atomicMax(&nonfinite, r);
+            }
+            put();
+            __syncthreads();
+            const int seen_bad = nonfinite, qb = qt * BQ + 32 * half;
+            next();
+            if (qb >= first) {       // (else: all of the block comes before the wavefront's keys)
+                f32x16 x[2];
+                weights(x);
+#pragma unroll
+                for (int i = 0; i < 16; ++i) {
+                    const bool seen = key <= qb + row_of(i, h);
+                    x[0][i] = seen ? x[0][i] : 0.f;
+                    x[1][i] = seen ? x[1][i] : 0.f;
+                }
+                add_columns<T, DP>(lds_g, 32 * half, x[0], dv, lane);
+                add_columns<T, DP>(lds_q, 32 * half, x[1], dk, lane);
+            }
+            if (seen_bad >= 0 && key <= qt * BQ + seen_bad) {       // (a key that such a query sees: its gradients are not finite)
+#pragma unroll
+                for (int b = 0; b < DB; ++b) {
+                    dk[b] += __builtin_nanf("");
+                    dv[b] += __builtin_nanf("");
+                }
+            }
+            __syncthreads();
+            if (t == 0) nonfinite = -1;
+        }
+        for (; qt < qt1; ++qt) {
+            __syncthreads();
+            put();
+            __syncthreads();
+            next();
+            f32x16 x[2];
+            weights(x);
+            add_columns<T, DP>(lds_g, 32 * half, x[0], dv, lane);
+            add_columns<T, DP>(lds_q, 32 * half, x[1], dk, lane);
+        }
+    }
+    auto join = [&](f32x16 (&x)[DB]) {
+        float *mine = (float *)lds + (wave & 3) * DB * 16 * 64 + lane;
+        __syncthreads();
+        if (half) {
+#pragma unroll
+            for (int b = 0; b < DB; ++b)
+#pragma unroll
+                for (int i = 0; i < 16; ++i) mine[(b * 16 + i) * 64] = x[b][i];
+        }
+        __syncthreads();
+        if (!half) {
+#pragma unroll
+            for (int b = 0; b < DB; ++b)
+#pragma unroll
+                for (int i = 0; i < 16; ++i) x[b][i] += mine[(b * 16 + i) * 64];
+        }
+    };
+    join(dk);
+    join(dv);
+    if (half || key >= w.length) return;
+    if (p.parts > 1) {
+        float *to = p.partial + (((int64_t)(w.start + key) * p.kv_heads + kvh) * p.parts + part) * 2 * DP;
+        store_row<float>(to, dk, 1.f, DP, lane);
+        store_row<float>(to + DP, dv, 1.f, DP, lane);
+    } else {
         store_row<T>((T *)(p.d_k.p + (int64_t)(w.start + key) * p.d_k.ts + kvh * p.d_k.hs), dk, p.scale, d, lane);
         store_row<T>((T *)(p.d_v.p + (int64_t)(w.start + key) * p.d_v.ts + kvh * p.d_v.hs), dv, 1.f, d, lane);
     }

@@ -22,7 +22,8 @@ SEQ_API int taco_attention_backward(const taco_attention_args *a, void *stream) 
             attention_dkv_kernel<T, DP, 1><<<grid_kv, 64, 0, s>>>(p);
         } else {
             attention_dq_kernel<T, DP, 4><<<grid, 256, 0, s>>>(p);
-            attention_dkv_kernel<T, DP, 4><<<grid_kv.x * p.parts, 256, 0, s>>>(p);
+            if constexpr (keys_in_lds<T, DP>) attention_dkv_pair_kernel<T, DP><<<grid_kv.x * p.parts, 512, 0, s>>>(p);
+            else attention_dkv_kernel<T, DP, 4><<<grid_kv.x * p.parts, 256, 0, s>>>(p);
             if (p.parts > 1) attention_sum_kernel<T, DP><<<grid_kv, 256, 0, s>>>(p);
         }
         return launched("taco_attention_backward");

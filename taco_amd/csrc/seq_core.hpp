@@ -131,6 +131,13 @@ template <typename T, int NS, typename A> __device__ __forceinline__ void mma_ro
     }
 }
 
+// the value itself, but not known to be the same from one turn of a loop to the next: what is computed from it is computed again each time instead of being
+// kept in registers that the loop has no room for
+__device__ __forceinline__ int afresh(int x) {
+    asm volatile("" : "+v"(x));
+    return x;
+}
+
 // ---- Global memory.  A buffer descriptor covers the rows of one tile that exist; what lies outside reads as zero, so no lane branches and padding rows and
 // padding columns cost nothing.  The base is 64 bits and moves with the tile, offsets inside it are 32.
 typedef __amdgpu_buffer_rsrc_t rsrc;
