@@ -99,7 +99,7 @@ __global__ __launch_bounds__(64 * NW, (waves_forward<T, DP, NW>)) void attention
 
     f32x16 o[DB];
     clear(o);
-    float m = -__builtin_inff(), l = 0.f;
+    float m = -__builtin_inff(), mu = -__builtin_inff(), l = 0.f;        // the running maximum, as it is and in the exponent's unit, and the sum
     const int last = p.causal ? min(w.length, w.first + BM) - 1 : w.length - 1;
     const int limit = p.causal ? row : w.length - 1;       // the last key this lane's query sees
     auto scores = [&](f32x16 (&s)[NB]) {
@@ -119,20 +119,21 @@ __global__ __launch_bounds__(64 * NW, (waves_forward<T, DP, NW>)) void attention
 #pragma unroll
             for (int i = 0; i < 16; ++i) mx = fmaxf(mx, s[n][i]);
         mx = fmaxf(mx, other_half(mx));
-        const float mn = fmaxf(m, mx), mu = mn == -__builtin_inff() ? 0.f : mn * c;
-        if (__any(mn > m)) {
-            float a = exp2_(m * c - mu);
+        if (__any(mx > m)) {
+            m = fmaxf(m, mx);
+            const float next = rounded(m * c), a = next == mu ? 1.f : exp2_(mu - next);
+            mu = next;
             l *= a;
 #pragma unroll
             for (int b = 0; b < DB; ++b) o[b] *= a;
-            m = mn;
         }
+        const float sub = mu == -__builtin_inff() ? 0.f : mu;
         float sum[4] = {0.f, 0.f, 0.f, 0.f};
 #pragma unroll
         for (int n = 0; n < NB; ++n)
 #pragma unroll
             for (int i = 0; i < 16; ++i) {
-                s[n][i] = exp2_(s[n][i] * c - mu);
+                s[n][i] = exp2_(s[n][i] * c - sub);
                 sum[i % 4] += s[n][i];
             }
         l += (sum[0] + sum[1]) + (sum[2] + sum[3]);
@@ -202,7 +203,7 @@ __global__ __launch_bounds__(64 * NW, (waves_forward<T, DP, NW>)) void attention
     l += other_half(l);
     if (row < w.length) {
         store_row<T>((T *)(p.o.p + (int64_t)(w.start + row) * p.o.ts + head * p.o.hs), o, l == 0.f ? 0.f : 1.f / l, d, lane);
-        if (h == 0) p.lse[(int64_t)(w.start + row) * p.heads + head] = m * p.scale + log2_(l) * LN2;
+        if (h == 0) p.lse[(int64_t)(w.start + row) * p.heads + head] = (mu + log2_(l)) * LN2;
     }
 }
 

@@ -79,7 +79,7 @@ __global__ __launch_bounds__(64 * NW, sizeof(T) == 2 ? 2 : 1) void attention_ste
 
     f32x16 o[DB];
     clear(o);
-    float m = -__builtin_inff(), l = 0.f;
+    float m = -__builtin_inff(), mu = -__builtin_inff(), l = 0.f;        // the running maximum, as it is and in the exponent's unit, and the sum
     int t0 = begin + 32 * wave;
     Place now{0, 0, false}, next{0, 0, false};
     if (t0 < end) {
@@ -106,19 +106,18 @@ __global__ __launch_bounds__(64 * NW, sizeof(T) == 2 ? 2 : 1) void attention_ste
 #pragma unroll
         for (int i = 1; i < 16; ++i) mx = fmaxf(mx, s[0][i]);
         mx = fmaxf(mx, other_half(mx));
-        const float mn = fmaxf(m, mx), mu = mn == -__builtin_inff() ? 0.f : mn * c;
-        if (__any(mn > m)) {
-            const float a = exp2_(m * c - mu);
+        if (__any(mx > m)) {
+            m = fmaxf(m, mx);
+            const float next = rounded(m * c), a = next == mu ? 1.f : exp2_(mu - next);
+            mu = next;
             l *= a;
 #pragma unroll
-            for (int x = 0; x < DB; ++x)
-#pragma unroll
-                for (int i = 0; i < 16; ++i) o[x][i] *= a;
-            m = mn;
+            for (int x = 0; x < DB; ++x) o[x] *= a;
         }
+        const float sub = mu == -__builtin_inff() ? 0.f : mu;
 #pragma unroll
         for (int i = 0; i < 16; ++i) {
-            s[0][i] = exp2_(s[0][i] * c - mu);
+            s[0][i] = exp2_(s[0][i] * c - sub);
             l += s[0][i];
         }
         put(vx);
@@ -147,7 +146,7 @@ __global__ __launch_bounds__(64 * NW, sizeof(T) == 2 ? 2 : 1) void attention_ste
             for (int i = 0; i < 16; i += 4)
                 *(f32x4 *)(so + (wave * cols + col) * DP + 32 * x + row_of(i, h)) = f32x4{o[x][i], o[x][i + 1], o[x][i + 2], o[x][i + 3]};
         if (h == 0) {
-            sm[(wave * cols + col) * 2] = m;
+            sm[(wave * cols + col) * 2] = mu;
             sm[(wave * cols + col) * 2 + 1] = l;
         }
     }
@@ -160,7 +159,7 @@ __global__ __launch_bounds__(64 * NW, sizeof(T) == 2 ? 2 : 1) void attention_ste
         f32x4 a{0, 0, 0, 0};
 #pragma unroll
         for (int y = 0; y < NW; ++y) {
-            const float my = sm[(y * cols + g) * 2], f = my == -__builtin_inff() ? 0.f : exp2_((my - M) * c);
+            const float my = sm[(y * cols + g) * 2], f = my == -__builtin_inff() ? 0.f : exp2_(my - M);
             L += sm[(y * cols + g) * 2 + 1] * f;
             a += *(const f32x4 *)(so + (y * cols + g) * DP + x) * f;
         }
@@ -195,7 +194,6 @@ __global__ __launch_bounds__(64) void attention_join_kernel(StepParams p) {
     const int b = blockIdx.x / p.heads, head = blockIdx.x % p.heads, lane = threadIdx.x, x = lane % W * 4, s = lane / W;
     const int n = pieces_of(keys_of(p.lengths[b], p.table_width, p.page_size, p.k_new.p != nullptr), p.piece);
     const int64_t at = (int64_t)blockIdx.x * p.pieces;
-    const float c = p.scale * LOG2E;
     float M = -__builtin_inff();
     for (int i = lane; i < n; i += 64) M = fmaxf(M, p.part_ml[(at + i) * 2]);
 #pragma unroll
@@ -203,7 +201,7 @@ __global__ __launch_bounds__(64) void attention_join_kernel(StepParams p) {
     float L = 0.f;
     f32x4 a{0, 0, 0, 0};
     for (int i = s; i < n; i += S) {
-        const float m = p.part_ml[(at + i) * 2], f = m == -__builtin_inff() ? 0.f : exp2_((m - M) * c);
+        const float m = p.part_ml[(at + i) * 2], f = m == -__builtin_inff() ? 0.f : exp2_(m - M);
         L += p.part_ml[(at + i) * 2 + 1] * f;
         a += *(const f32x4 *)(p.part_o + (at + i) * DP + x) * f;
     }

@@ -57,6 +57,12 @@ template <int N> __device__ __forceinline__ void clear(f32x16 (&x)[N]) {
 __device__ __forceinline__ float other_half(float x) { return __shfl_xor(x, 32); }
 __device__ __forceinline__ float exp2_(float x) { return __builtin_amdgcn_exp2f(x); }
 __device__ __forceinline__ float log2_(float x) { return __builtin_amdgcn_logf(x); }
+// a product as it was rounded, wherever it is used (not fused into one of its uses and rounded apart from the others).  The softmax keeps its maximum that way:
+// the factor that joins two maxima is then exactly 1 where a row's own has not changed, and sums do not drift by a rounding each time another row's does.
+__device__ __forceinline__ float rounded(float x) {
+    asm("" : "+v"(x));
+    return x;
+}
 constexpr float LOG2E = 1.4426950408889634f, LN2 = 0.6931471805599453f;
 
 // ---- LDS tiles: rows of DP elements (the head dimension padded with zeros to 32, 64 or 128), 16-byte chunks exchanged inside each row by an XOR that

@@ -45,9 +45,7 @@ template <typename T, int DP, int C> __device__ __forceinline__ void add_outer(c
         const f32x4 t0 = *(const f32x4 *)(tail + 16 * e + 4 * (lane >> 5)), t1 = *(const f32x4 *)(tail + 16 * e + 8 + 4 * (lane >> 5));
 #pragma unroll
         for (int j = 0; j < 8; ++j) {
-            float x = (float)v[j] * (j < 4 ? t0[j % 4] : t1[j % 4]);
-            // x is one float32 from here on: a multiplication fused into one of its uses and not into the other rounds them apart on a tie
-            asm("" : "+v"(x));
+            float x = rounded((float)v[j] * (j < 4 ? t0[j % 4] : t1[j % 4]));      // (fused into one of its uses and not into the other: apart on a tie)
 #pragma unroll
             for (int n = 0; n < PARTS; ++n) {
                 p[n][j] = (T)x;
