@@ -7,8 +7,8 @@
  *
  * Ownership, errors and streams as in taco_env.h: the caller allocates every buffer, the library borrows DEVICE pointers for the call, enqueues on
  * the caller's stream (whose device has to be the current one), never synchronises, allocates or throws.  Every function returns TACO_SEQ_OK or
- * a negative status; taco_sequence_last_error() returns a thread-local message.  Everything may be captured into a HIP graph.  No atomics: the
- * same call gives the same bits.
+ * a negative status; taco_sequence_last_error() returns a thread-local message.  Everything may be captured into a HIP graph.  No sum depends on an
+ * order that is not fixed: the same call gives the same bits.
  *
  * Tensors: `ptr` 16-byte aligned, the head dimension contiguous, token and head strides in ELEMENTS, multiples of 16 bytes.  All of one dtype
  * unless said otherwise.  dim: a multiple of 8, 8 .. 128.  Sums, softmax statistics and states are float32.

@@ -31,9 +31,9 @@ __global__ __launch_bounds__(64 * NW, sizeof(T) == 2 ? 2 : 1) void attention_ste
     const int G = p.heads / p.kv_heads, g0 = 32 * blk, cols = min(32, G - g0), head0 = kvh * G + g0;
     const bool joins = p.k_new.p != nullptr;
     const int len = p.lengths[b], keys = keys_of(len, p.table_width, p.page_size, joins);
-    const int begin = blockIdx.y * p.piece;
-    if (blockIdx.y > 0 && begin >= keys) return;
-    const int end = max(0, min(keys, begin + p.piece));
+    const int64_t from = (int64_t)blockIdx.y * p.piece;         // (a table may have room for more than 2^31 tokens)
+    if (blockIdx.y > 0 && from >= keys) return;
+    const int begin = (int)from, end = (int)(from + p.piece < keys ? from + p.piece : max(keys, 0));
     const int32_t *table = p.table + b * p.table_stride;
     char *mine = lds + wave * 32 * tile::ROW;
     const float c = p.scale * LOG2E;

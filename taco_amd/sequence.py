@@ -110,6 +110,10 @@ def _call(f, args, device):
         raise _lib.TacoError(f"libtaco_sequence: status {rc}: {load().taco_sequence_last_error().decode()}")
 
 
+# what a call writes into a caller's tensor is a change in place for autograd too: a graph that has saved it refuses to run backward through it
+_written = torch.autograd.graph.increment_version
+
+
 # ---- checks shared by the calls (messages are made where a check fails: the host side of a call is most of a short one's time) ---------
 
 def _check_rows(what, q, *others):
@@ -308,6 +312,8 @@ def _attention_forward(q, k, v, seqs, causal, scale, out):
     total, device = seqs.total, q.device
     o = _empty(q.shape, total, q.dtype, device) if out is None else out
     lse = _empty(q.shape[:2], total, torch.float32, device)
+    if out is not None:
+        _written(out)
     if total:
         _launch_tiles(_attention_args(q, k, v, o, lse, seqs, causal, scale), seqs, device, False)
     return q, k, v, o, lse
@@ -441,6 +447,7 @@ def attention_step(q, k, v, k_pages, v_pages, page_table, lengths, scale=None, o
         ws = torch.empty(need, dtype=torch.uint8, device=device)
         a.workspace, a.workspace_bytes = ws.data_ptr(), need
     _call(lib.taco_attention_step, a, device)
+    _written((out,) if k is None else (out, k_pages, v_pages))
     return out
 
 
@@ -571,4 +578,5 @@ def linear_attention_step(q, k, v, log_decay, state, reset=None, scale=None, out
     a = LinearStepArgs(_tensor(q), _tensor(k), _tensor(v), _tensor(out), log_decay.data_ptr(), state.data_ptr(), None if reset is None else reset.data_ptr(),
                        0 if reset is None else _RESET_BYTES[reset.dtype], B, H, d, code, scale)
     _call(load().taco_linear_attention_step, a, device)
+    _written((out, state))
     return out

@@ -69,12 +69,13 @@ def test_attention_in_tiles_of_128_rows(dtype, d):
 
 
 @pytest.mark.parametrize("dtype", DTYPES)
-def test_attention_group_in_parts(dtype):
+@pytest.mark.parametrize("d", [24, 128])
+def test_attention_group_in_parts(dtype, d):
     """one long sequence, few key-value heads: the group's heads are shared out, and their sums joined"""
     lens = [700, 129]
     seqs = S().Packed(lens, "cuda:0")
     assert seqs._parts(64, 32, True) > 1 and seqs._tiles(64)[0][0] == 128
-    check_attention(64, 2, 24, lens, dtype)
+    check_attention(64, 2, d, lens, dtype)
 
 
 @pytest.mark.parametrize("dtype", DTYPES)
@@ -90,11 +91,10 @@ def test_attention_scale_and_large_scores():
 
 
 @pytest.mark.parametrize("dtype", DTYPES)
-@pytest.mark.parametrize("H,lens,bad", [(2, [70, 150, 33], 41), (130, [70, 150, 33], 41), (2, [9, 30, 32], 11)])
+@pytest.mark.parametrize("H,d,lens,bad", [(2, 64, [70, 150, 33], 41), (130, 64, [70, 150, 33], 41), (130, 128, [70, 150, 33], 41), (2, 64, [9, 30, 32], 11)])
 @pytest.mark.parametrize("poison", [float("nan"), float("inf"), -float("inf")])
-def test_hidden_tokens_have_no_influence(dtype, H, lens, bad, poison):
+def test_hidden_tokens_have_no_influence(dtype, H, d, lens, bad, poison):
     """a token that diverges at one step of a sequence: the steps before it, and the other sequences, get the bits they get without it, forward and backward"""
-    d = 64
     T = sum(lens)
     at = lens[0] + bad
     q, k, v, g = (randn(T, H, d, dtype=dtype, seed=i) for i in range(4))
@@ -269,7 +269,7 @@ def want_step(q, keys, k, v, scale):
     o, bound = torch.zeros(B, H, d, dtype=torch.float64), torch.zeros(B, H, d, dtype=torch.float64)
     u, low = R.half_step(q.dtype), R.low_step(q.dtype)
     for b in range(B):
-        K, V = (torch.cat([x, y[b][None].cpu()]) if y is not None else x for x, y in zip(keys[b], (k, v)))
+        K, V = (torch.cat([x, y[b][None].cpu()]) if y[b] is not None else x for x, y in zip(keys[b], (k, v)))
         G = H // K.shape[1]
         for h in range(H if len(K) else 0):
             r = R.attention(q[b, h][None].double().cpu(), K[:, h // G].double(), V[:, h // G].double(), scale, False)
@@ -610,3 +610,37 @@ def test_the_same_bits_every_time():
     first = run()
     for _ in range(3):
         assert all(torch.equal(a, b) for a, b in zip(first, run()))
+
+
+def test_what_is_written_in_place_counts_as_changed():
+    """a state, a cache or an output that a graph has saved: backward refuses instead of using what a later call wrote there"""
+    s = S()
+    x = [randn(8, 2, 32, seed=i).requires_grad_() for i in range(3)]
+    decay, state, seqs = torch.full((2,), -0.1, device="cuda"), randn(4, 2, 32, 32), s.Packed([2, 2, 2, 2], "cuda:0")
+    o, _ = s.linear_attention(*x, decay, seqs, state=state)
+    tok = [randn(4, 2, 32, seed=9 + i) for i in range(3)]
+    s.linear_attention_step(*tok, decay, state)
+    with pytest.raises(RuntimeError, match="modified by an inplace operation"):
+        o.sum().backward()
+    pages = torch.zeros(4, 4, 2, 32, device="cuda")
+    w = torch.ones(1, device="cuda", requires_grad=True)
+    y = (pages * w).sum()
+    s.attention_step(*tok, pages, pages.clone(), torch.arange(4, dtype=torch.int32, device="cuda").view(4, 1), torch.zeros(4, dtype=torch.int32, device="cuda"))
+    with pytest.raises(RuntimeError, match="modified by an inplace operation"):
+        y.backward()
+    with torch.inference_mode():
+        z = [t.detach().clone() for t in tok]
+        assert torch.equal(s.linear_attention_step(*z, decay, torch.zeros(4, 2, 32, 32, device="cuda")), s.linear_attention_step(*tok, decay, torch.zeros(4, 2, 32, 32, device="cuda")))
+
+
+def test_attention_step_room_past_32_bits():
+    """a table with room for more than 2^31 tokens (one page, named over and over): a short row reads only its own"""
+    H, d, page = 2, 32, 1 << 20
+    kp, vp = (torch.zeros(1, page, 1, d, dtype=torch.float16, device="cuda") for _ in range(2))
+    kp[0, :40], vp[0, :40] = randn(40, 1, d, dtype=torch.float16, seed=1), randn(40, 1, d, dtype=torch.float16, seed=2)
+    q = randn(1, H, d, dtype=torch.float16, seed=3)
+    n = torch.tensor([40], dtype=torch.int32, device="cuda")
+    wide = torch.zeros(1, 4096, dtype=torch.int32, device="cuda")
+    got = S().attention_step(q, None, None, kp, vp, wide, n)
+    near(got, *want_step(q, [(kp[0, :40].cpu(), vp[0, :40].cpu())], [None], [None], 1 / math.sqrt(d)), "room past 2^31")
+    assert (S().attention_step(q, None, None, kp, vp, wide, torch.zeros_like(n)) == 0).all()
