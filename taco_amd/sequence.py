@@ -256,14 +256,29 @@ class Packed:
         return group
 
     def _segments(self, work):
-        """(segments, first segment of each sequence, count) for `work` = heads x products.  A workgroup fills a CU, so pieces of half a CU's share of all tokens
-        (at least 256) even out what sequences of different lengths leave; a sequence is cut into equal pieces where it is longer than one and a half."""
-        size = max(256, -(-self.total * work // (512 * 64)) * 64)
-        key = ("segments", size)
+        """(segments, first segment of each sequence, count) for `work` = heads x products: workgroups for each segment, one to a CU.  Fewer, longer segments leave CUs
+        idle; each cut costs a second reading of its k and v and the state's way through memory and back.  Of some lengths (at least 256 tokens; sequences
+        are cut into equal pieces) the one with the least estimate is taken, in tokens of a CU's time: the longest segment if all run at once, else a CU's
+        share and half the longest; a third for a token that is read again; 160 for a state (linear_prompts: 200 us in two rounds of pieces, 234 in
+        three)."""
+        got = self._lists.get(("segments", work))
+        if got is not None:
+            return self._kept(("segments", work), None)
+
+        def pieces(size):
+            return np.maximum(-(-self.lengths // size), 1)
+
+        def estimate(size):
+            n = pieces(size)
+            longest, share = (self.lengths / n).max(initial=0), self.total * work / 256
+            again = (self.lengths * (n - 1) / n).sum() / 3 + 160 * n[n > 1].sum()
+            return (longest if n.sum() * work <= 256 else share + longest / 2) + again * work / 256
 
         def make():
-            n = np.where(self.lengths <= size + size // 2, 1, -(-self.lengths // size))
-            if len(n) and n.sum() > len(n) and len(n) * work > 65535:      # (the joining launch's limit; so many sequences fill the CUs by themselves)
+            uncut = max(self._longest, 256)
+            sizes = {max(256, -(-int(self.total * work / (256 * rounds)) // 64) * 64) for rounds in (0.75, 0.9, 1, 1.2, 1.5, 1.75, 2, 2.5, 3, 4)}
+            n = pieces(min([uncut] + sorted(sizes, reverse=True), key=estimate))
+            if n.sum() > len(n) and len(n) * work > 65535:      # (the joining launch's limit; so many sequences fill the CUs by themselves)
                 n = np.ones_like(n)
             first = np.concatenate([[0], np.cumsum(n)])
             of = np.repeat(np.arange(len(n)), n)
@@ -272,7 +287,7 @@ class Packed:
             at = index * step
             cols = [of, self.starts[of], self.lengths[of], at, np.minimum(step, self.lengths[of] - at), index, index * 0, index * 0]
             return [np.stack(cols, 1).astype(np.int32).reshape(-1, 8), first.astype(np.int32), len(of)]
-        return self._kept(key, make)
+        return self._kept(("segments", work), make)
 
 
 # ---- attention over packed sequences -----------------------------------------------------------------------------------------------
