@@ -36,7 +36,7 @@ static int run(const taco_linear_attention_args *a, LinearParams &p, int modes, 
         constexpr int DP = decltype(dp)::value;
         const dim3 grid((unsigned)p.n_segments, (unsigned)p.heads, (unsigned)modes);
         if (p.carry) {
-            linear_kernel<T, DP, true><<<grid, 2 * DP, 0, (hipStream_t)stream>>>(p);
+            linear_kernel<T, DP, true><<<grid, 2 * DP * (chunk_of<T> / 32), 0, (hipStream_t)stream>>>(p);
             linear_scan_kernel<DP><<<dim3(DP * DP / 256, (unsigned)(p.n_sequences * p.heads), (unsigned)modes), 256, 0, (hipStream_t)stream>>>(p);
         }
         linear_kernel<T, DP, false><<<grid, 4 * DP, 0, (hipStream_t)stream>>>(p);

@@ -34,15 +34,15 @@ __device__ __forceinline__ float decay2(const float *log_decay, int head) {
     return x < -1e30f ? -1e30f : x;
 }
 
-// acc[b] += K^T (V * tail), a chunk's part of the state.  tail decays per token, so V * tail has float32's 24 bits; it goes through the 16-bit product in
+// acc[b] += K^T (V * tail), C tokens' part of the state, from row0.  tail decays per token, so V * tail has float32's 24 bits; it goes through the 16-bit product in
 // parts that add up to it, and the state stays as exact as float32 sums: bf16 in three parts of 8 bits; fp16 in two of 11 (the second scaled by 2^11, with
 // a sum of its own, so that small values do not fall below fp16's range).
-template <typename T, int DP, int C> __device__ __forceinline__ void add_outer(const char *lds_k, const char *lds_v, const float *tail, int col0, f32x16 (&acc)[DP / 32], int lane) {
+template <typename T, int DP, int C> __device__ __forceinline__ void add_outer(const char *lds_k, const char *lds_v, const float *tail, int row0, int col0, f32x16 (&acc)[DP / 32], int lane) {
     typedef Tile<T, DP> tile;
     constexpr int E = C / 16, PARTS = sizeof(T) == 4 ? 1 : __is_same(T, f16) ? 2 : 3;
     auto parts = [&](int e, frag<T> (&p)[PARTS]) {
-        const frag<T> v = tile::cols(lds_v, 16 * e, col0, lane);
-        const f32x4 t0 = *(const f32x4 *)(tail + 16 * e + 4 * (lane >> 5)), t1 = *(const f32x4 *)(tail + 16 * e + 8 + 4 * (lane >> 5));
+        const frag<T> v = tile::cols(lds_v, row0 + 16 * e, col0, lane);
+        const f32x4 t0 = *(const f32x4 *)(tail + row0 + 16 * e + 4 * (lane >> 5)), t1 = *(const f32x4 *)(tail + row0 + 16 * e + 8 + 4 * (lane >> 5));
 #pragma unroll
         for (int j = 0; j < 8; ++j) {
             float x = rounded((float)v[j] * (j < 4 ? t0[j % 4] : t1[j % 4]));      // (fused into one of its uses and not into the other: apart on a tie)
@@ -64,7 +64,7 @@ template <typename T, int DP, int C> __device__ __forceinline__ void add_outer(c
             clear(low);
 #pragma unroll
             for (int e = 0; e < E; ++e) {
-                const frag<T> k = tile::cols(lds_k, 16 * e, 32 * b, lane);
+                const frag<T> k = tile::cols(lds_k, row0 + 16 * e, 32 * b, lane);
                 acc[b] = mma(k, p[e][0], acc[b]);
                 low[0] = mma(k, p[e][1], low[0]);
             }
@@ -75,7 +75,7 @@ template <typename T, int DP, int C> __device__ __forceinline__ void add_outer(c
         for (int e = 0; e < E; ++e) {
             frag<T> p[PARTS], k[DP / 32];
 #pragma unroll
-            for (int b = 0; b < DP / 32; ++b) k[b] = tile::cols(lds_k, 16 * e, 32 * b, lane);
+            for (int b = 0; b < DP / 32; ++b) k[b] = tile::cols(lds_k, row0 + 16 * e, 32 * b, lane);
             __builtin_amdgcn_sched_barrier(0);
             parts(e, p);
             // (the same block's sums apart: a product does not wait for the one before it)
@@ -92,12 +92,13 @@ template <typename T, int DP, int C> __device__ __forceinline__ void add_outer(c
 // other makes the outputs from the state before the chunk (P^T = K Q^T with the decays, O^T = V^T P^T + S^T Q^T), which the first leaves for it in LDS as
 // the operand it will be.  One wavefront for both would need more registers than two on a SIMD can have, and then nothing hides its waits.
 // P and S are rounded to the inputs' type for their products, the state itself never is.
-// STATES: only the state that the segment makes from nothing, for `carry`.
+// STATES: only the state that the segment makes from nothing, for `carry`; there are fewer of these than CUs, so each chunk is shared out to QB keepers, 32
+// tokens each, whose sums meet in LDS at the end.
 template <typename T> constexpr int chunk_of = sizeof(T) == 4 ? 32 : 64;        // (float32: the tiles and the state's copy have to fit 160 KB of LDS)
 template <typename T, int DP, bool STATES>
-__global__ __launch_bounds__(STATES ? 2 * DP : 4 * DP, 2) void linear_kernel(LinearParams p) {
+__global__ __launch_bounds__(STATES ? 2 * DP * (chunk_of<T> / 32) : 4 * DP, 2) void linear_kernel(LinearParams p) {
     typedef Tile<T, DP> tile;
-    constexpr int C = chunk_of<T>, NT = STATES ? 2 * DP : 4 * DP, NS = DP / 16, DB = DP / 32, QB = C / 32;
+    constexpr int C = chunk_of<T>, NT = STATES ? 2 * DP * (C / 32) : 4 * DP, NS = DP / 16, DB = DP / 32, QB = C / 32;
     __shared__ __attribute__((aligned(16))) char lds_k[C * tile::ROW], lds_v[C * tile::ROW], lds_q[STATES ? 16 : C * tile::ROW];
     __shared__ __attribute__((aligned(16))) char lds_s[STATES ? 16 : DP * tile::ROW];      // the state before the chunk, transposed
     __shared__ __attribute__((aligned(16))) float tail[C], to_end[32];      // decay from each token to the last of the chunk; of 32 tokens
@@ -196,7 +197,8 @@ __global__ __launch_bounds__(STATES ? 2 * DP : 4 * DP, 2) void linear_kernel(Lin
             const float gn = exp2_(ld * (n - 1 + m.shift));
 #pragma unroll
             for (int b = 0; b < DB; ++b) s[b] *= gn;
-            add_outer<T, DP, C>(lds_k, lds_v, tail, 32 * slice, s, lane);
+            if constexpr (STATES) add_outer<T, DP, 32>(lds_k, lds_v, tail, 32 * (wave / DB), 32 * slice, s, lane);
+            else add_outer<T, DP, C>(lds_k, lds_v, tail, 0, 32 * slice, s, lane);
             if (!STATES && nonfinite == c0) {
                 const bool bad = first_nonfinite_token(c0, n) < C;
 #pragma unroll
@@ -209,6 +211,24 @@ __global__ __launch_bounds__(STATES ? 2 * DP : 4 * DP, 2) void linear_kernel(Lin
             }
         }
         if (STATES) {
+            if constexpr (QB == 2) {
+                static_assert(DB * 16 * 64 * sizeof(float) <= sizeof(lds_k), "a block of every keeper's");
+                float *sums = (float *)lds_k + slice * 16 * 64 + lane;
+#pragma unroll
+                for (int b = 0; b < DB; ++b) {
+                    __syncthreads();
+                    if (wave >= DB) {
+#pragma unroll
+                        for (int i = 0; i < 16; ++i) sums[i * 64] = s[b][i];
+                    }
+                    __syncthreads();
+                    if (wave < DB) {
+#pragma unroll
+                        for (int i = 0; i < 16; ++i) s[b][i] += sums[i * 64];
+                    }
+                }
+                if (wave >= DB) return;
+            }
 #pragma unroll
             for (int b = 0; b < DB; ++b)
 #pragma unroll
