@@ -56,7 +56,7 @@ typedef struct taco_attention_args {
     taco_seq_tensor d_o, d_q, d_k, d_v;
     float *delta;                       /* workspace [tokens][heads] */
     int32_t parts;                      /* 128-row tiles: a key-value head's group of query heads in that many parts (a divisor of heads / kv_heads), each a
-                                           workgroup of its own; more than 1 needs the workspace [tokens][kv_heads][parts][2][dim padded to 32, 64 or 128] */
+                                           workgroup of its own; more than 1 needs the workspace [tokens][kv_heads][parts][2][dim rounded up to a multiple of 32] */
     float *partial;
 } taco_attention_args;
 int taco_attention(const taco_attention_args *a, void *stream);
@@ -91,7 +91,7 @@ int taco_attention_step(const taco_attention_step_args *a, void *stream);
 /* ---- Linear attention with a decay for each head: S_t = g S_{t-1} + k_t v_t^T, o_t = scale * q_t S_t, g = exp(log_decay[head]).
  * state0, state_last: float32 [sequences][heads][dim][dim] (key dimension first), contiguous; NULL: zeros / not wanted.  They must not overlap.
  * The work list: DEVICE array of segments, those of one sequence behind one another in order.  A sequence of no tokens has one segment of none.
- * n_segments > n_sequences needs the workspace (float32 [n_segments][heads][dim padded to 32, 64 or 128]^2). */
+ * n_segments > n_sequences needs the workspace (float32 [n_segments][heads][dim rounded up to a multiple of 32]^2). */
 typedef struct taco_seq_segment { int32_t sequence, start, length, first, count, index, pad0, pad1; } taco_seq_segment;
                         /* start, length: the sequence's tokens; first, count: the segment's, counted in the sequence; index: its number in the sequence */
 typedef struct taco_linear_attention_args {

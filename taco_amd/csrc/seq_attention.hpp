@@ -32,8 +32,8 @@ __device__ __forceinline__ void locate(int block, int heads, int &tile, int &hea
 template <typename T, int DP, int NW> constexpr int waves_forward = sizeof(T) == 4 ? (DP == 32 ? 2 : 1) : DP == 32 ? 4 : DP == 64 || NW == 4 ? 2 : 1;
 template <typename T, int DP, int NW> constexpr int waves_dq = sizeof(T) == 4 ? (DP == 32 ? 2 : 1) : DP <= 64 || NW == 4 ? 2 : 1;
 template <typename T, int DP> constexpr int waves_dkv = sizeof(T) == 4 ? (DP == 32 ? 2 : 1) : DP <= 64 ? 2 : 1;
-// The next tiles travel in registers while these are used, except where that would spill: float32 rows of 128 hold half the registers as operands already.
-template <typename T, int DP> constexpr bool ahead = !(sizeof(T) == 4 && DP == 128);
+// The next tiles travel in registers while these are used, except where that would spill: wide float32 rows hold half the registers as operands already.
+template <typename T, int DP> constexpr bool ahead = !(sizeof(T) == 4 && DP >= 96);
 
 // (and there the compiler must not ask LDS for many operands at once either)
 template <typename T, int DP> __device__ __forceinline__ void in_order() {

@@ -187,10 +187,10 @@ __global__ __launch_bounds__(64 * NW, sizeof(T) == 2 ? 2 : 1) void attention_ste
     }
 }
 
-// The pieces of a row and head joined: one wavefront, DP / 4 lanes across the dimension, 256 / DP pieces side by side.
+// The pieces of a row and head joined: one wavefront, DP / 4 lanes across the dimension (32 for 96), the other lanes take other pieces.
 template <typename T, int DP>
 __global__ __launch_bounds__(64) void attention_join_kernel(StepParams p) {
-    constexpr int W = DP / 4, S = 64 / W;
+    constexpr int W = DP == 96 ? 32 : DP / 4, S = 64 / W;
     const int b = blockIdx.x / p.heads, head = blockIdx.x % p.heads, lane = threadIdx.x, x = lane % W * 4, s = lane / W;
     const int n = pieces_of(keys_of(p.lengths[b], p.table_width, p.page_size, p.k_new.p != nullptr), p.piece);
     const int64_t at = (int64_t)blockIdx.x * p.pieces;
@@ -203,7 +203,7 @@ __global__ __launch_bounds__(64) void attention_join_kernel(StepParams p) {
     for (int i = s; i < n; i += S) {
         const float m = p.part_ml[(at + i) * 2], f = m == -__builtin_inff() ? 0.f : exp2_(m - M);
         L += p.part_ml[(at + i) * 2 + 1] * f;
-        a += *(const f32x4 *)(p.part_o + (at + i) * DP + x) * f;
+        if (x < DP) a += *(const f32x4 *)(p.part_o + (at + i) * DP + x) * f;
     }
 #pragma unroll
     for (int i = W; i < 64; i <<= 1) {

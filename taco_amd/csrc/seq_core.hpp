@@ -65,16 +65,17 @@ __device__ __forceinline__ float rounded(float x) {
 }
 constexpr float LOG2E = 1.4426950408889634f, LN2 = 0.6931471805599453f;
 
-// ---- LDS tiles: rows of DP elements (the head dimension padded with zeros to 32, 64 or 128), 16-byte chunks exchanged inside each row by an XOR that
+// ---- LDS tiles: rows of DP elements (the head dimension padded with zeros to 32, 64, 96 or 128; 96 in the room of 128), 16-byte chunks exchanged inside each row by an XOR that
 // depends on the row.  256 bytes are one turn of the 64 banks.  A row-wise read (32 rows, the same chunk) wants 16 neighbouring rows in 16 different
 // chunk positions; a column-wise read (4 neighbouring rows, 64 bytes each) wants the four rows in different quarters.  flip() gives both.
 template <typename T, int DP> struct Tile {
     static constexpr int NC = DP * (int)sizeof(T) / 16;         // chunks of a row
     static constexpr int CE = 16 / (int)sizeof(T);              // elements of a chunk
-    static constexpr int ROW = NC * 16;                         // bytes of a row
+    static constexpr int ROOM = DP == 96 ? NC / 3 * 4 : NC;     // chunks that a row has room for, a power of two
+    static constexpr int ROW = ROOM * 16;                       // bytes of a row
     static __device__ __forceinline__ int flip(int r) {
-        if (NC == 4) return (r >> 2) & 3;
-        if (NC == 8) return ((r >> 1) & 1) << 2 | ((r >> 2) & 3);
+        if (ROOM == 4) return (r >> 2) & 3;
+        if (ROOM == 8) return ((r >> 1) & 1) << 2 | ((r >> 2) & 3);
         return (r & 3) << 2 | ((r >> 2) & 3);
     }
     static __device__ __forceinline__ int at(int r, int c) { return r * ROW + ((c ^ flip(r)) << 4); }

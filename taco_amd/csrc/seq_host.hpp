@@ -9,7 +9,7 @@ int fail(int code, const char *fmt, ...) __attribute__((format(printf, 2, 3), vi
 #define SEQ_NEED(cond, ...) do { if (!(cond)) return ::seq::fail(TACO_SEQ_ERR_INVALID_ARG, __VA_ARGS__); } while (0)
 
 inline int64_t size_of(int dtype) { return dtype == TACO_SEQ_F32 ? 4 : 2; }
-inline int padded_dim(int dim) { return dim <= 32 ? 32 : dim <= 64 ? 64 : 128; }
+inline int padded_dim(int dim) { return (dim + 31) / 32 * 32; }
 
 inline int check_dims(int heads, int kv_heads, int dim, int dtype) {
     SEQ_NEED(dtype >= TACO_SEQ_F32 && dtype <= TACO_SEQ_BF16, "dtype %d is none of TACO_SEQ_F32, TACO_SEQ_F16, TACO_SEQ_BF16", dtype);
@@ -44,7 +44,7 @@ inline int launched(const char *what) {
 // f(T(), dim padded as an integral constant) for the call's type and head size
 template <int N> struct Int { static constexpr int value = N; };
 template <typename F> int dispatch(int dtype, int dim, F f) {
-    auto by_dim = [&](auto type) { return dim <= 32 ? f(type, Int<32>()) : dim <= 64 ? f(type, Int<64>()) : f(type, Int<128>()); };
+    auto by_dim = [&](auto type) { return dim <= 32 ? f(type, Int<32>()) : dim <= 64 ? f(type, Int<64>()) : dim <= 96 ? f(type, Int<96>()) : f(type, Int<128>()); };
     return dtype == TACO_SEQ_F32 ? by_dim(float()) : dtype == TACO_SEQ_F16 ? by_dim(f16()) : by_dim(bf16());
 }
 

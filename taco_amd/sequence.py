@@ -360,7 +360,7 @@ class _Attention(torch.autograd.Function):
             H, Hk, d = q.shape[1], k.shape[1], q.shape[2]
             a.parts = 1 if H == Hk else seqs._parts(H, H // Hk, causal)
             if a.parts > 1:
-                partial = torch.empty((seqs.total, Hk, a.parts, 2, 32 if d <= 32 else 64 if d <= 64 else 128), dtype=torch.float32, device=q.device)
+                partial = torch.empty((seqs.total, Hk, a.parts, 2, -(-d // 32) * 32), dtype=torch.float32, device=q.device)
                 a.partial = partial.data_ptr()
             _launch_tiles(a, seqs, q.device, True)
         return dq, dk, dv, None, None, None

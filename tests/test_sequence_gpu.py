@@ -52,14 +52,14 @@ def check_attention(H, Hk, d, lens, dtype, causal=True, scale=None, seed=0, trai
 
 @pytest.mark.parametrize("dtype", DTYPES)
 @pytest.mark.parametrize("H,Hk,d,lens", [
-    (1, 1, 8, [1]), (2, 2, 32, [1, 2, 31, 32, 33]), (4, 2, 64, [5, 64, 1, 65, 17]), (6, 2, 80, [40, 3]), (8, 1, 128, [70, 1, 33]), (3, 3, 24, [0, 7, 0, 64]),
+    (1, 1, 8, [1]), (2, 2, 32, [1, 2, 31, 32, 33]), (4, 2, 64, [5, 64, 1, 65, 17]), (6, 2, 80, [40, 3]), (4, 2, 96, [70, 33, 20]), (8, 1, 128, [70, 1, 33]), (3, 3, 24, [0, 7, 0, 64]),
     (8, 8, 16, [128, 100])])
 def test_attention_and_its_gradients(dtype, H, Hk, d, lens):
     check_attention(H, Hk, d, lens, dtype)
 
 
 @pytest.mark.parametrize("dtype", DTYPES)
-@pytest.mark.parametrize("d", [32, 64, 128])
+@pytest.mark.parametrize("d", [32, 64, 96, 128])
 def test_attention_in_tiles_of_128_rows(dtype, d):
     """enough tiles that the wide form runs (256 and more, heads counted), with short sequences beside the long ones"""
     lens = [129, 64, 300, 1, 128]
@@ -279,7 +279,7 @@ def want_step(q, keys, k, v, scale):
 
 @pytest.mark.parametrize("dtype", DTYPES)
 @pytest.mark.parametrize("H,Hk,d,page,lens", [
-    (1, 1, 8, 1, [0]), (4, 4, 32, 8, [0, 1, 7, 8, 9, 31]), (8, 2, 64, 16, [129, 0, 63, 300]), (6, 3, 80, 24, [5, 47, 48, 200]), (40, 1, 128, 16, [33, 500]),
+    (1, 1, 8, 1, [0]), (4, 4, 32, 8, [0, 1, 7, 8, 9, 31]), (8, 2, 64, 16, [129, 0, 63, 300]), (6, 3, 80, 24, [5, 47, 48, 200]), (6, 3, 96, 24, [5, 200]), (40, 1, 128, 16, [33, 500]),
     (16, 4, 128, 64, [1000, 3]), (5, 5, 16, 3, [2, 100])])
 def test_attention_step(dtype, H, Hk, d, page, lens):
     kp, vp, table, lengths, keys = cache_of(lens, Hk, d, page, dtype)
@@ -299,9 +299,10 @@ def test_attention_step(dtype, H, Hk, d, page, lens):
 
 
 @pytest.mark.parametrize("dtype", DTYPES)
-def test_attention_step_in_pieces(dtype):
+@pytest.mark.parametrize("d", [32, 64, 80, 128])
+def test_attention_step_in_pieces(dtype, d):
     """tables wide enough that rows are split over workgroups: long rows, rows shorter than a piece, an empty one"""
-    lens, page, H, Hk, d = [2500, 0, 255, 256, 1023, 1], 16, 4, 2, 64
+    lens, page, H, Hk = [2500, 0, 255, 256, 1023, 1], 16, 4, 2
     kp, vp, table, lengths, keys = cache_of(lens, Hk, d, page, dtype, width=400)
     table[table == -7] = 2 ** 31 - 1        # entries behind a row's pages are never read as pages
     q, k, v = (randn(len(lens), h, d, dtype=dtype, seed=50 + h) for h in (H, Hk, Hk))
@@ -397,7 +398,7 @@ def check_linear(lens, H, d, dtype, with_state=True, train=True, decays=None, se
 
 
 @pytest.mark.parametrize("dtype", DTYPES)
-@pytest.mark.parametrize("lens,H,d", [([1], 1, 8), ([1, 2, 31, 32, 33], 2, 32), ([63, 64, 65, 0, 130], 3, 64), ([100, 7], 2, 80), ([129, 200], 2, 128)])
+@pytest.mark.parametrize("lens,H,d", [([1], 1, 8), ([1, 2, 31, 32, 33], 2, 32), ([63, 64, 65, 0, 130], 3, 64), ([100, 7], 2, 80), ([130, 5], 2, 96), ([129, 200], 2, 128)])
 def test_linear_attention_and_its_gradients(dtype, lens, H, d):
     check_linear(lens, H, d, dtype)
 
@@ -409,6 +410,7 @@ def test_linear_attention_in_segments(dtype):
     seqs = S().Packed(lens, "cuda:0")
     assert seqs._segments(2)[2] > len(lens)
     check_linear(lens, 2, 40, dtype)
+    check_linear([300, 600], 2, 80, dtype)
     check_linear(lens, 2, 32, dtype, with_state=False)
 
 
