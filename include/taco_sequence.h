@@ -54,7 +54,7 @@ typedef struct taco_attention_args {
     float scale;                        /* > 0 */
     /* backward only: */
     taco_seq_tensor d_o, d_q, d_k, d_v;
-    float *delta;                       /* workspace [tokens][heads] */
+    float *delta;                       /* workspace [tokens][heads]: scale * rowsum(d_o o) */
     int32_t parts;                      /* 128-row tiles: a key-value head's group of query heads in that many parts (a divisor of heads / kv_heads), each a
                                            workgroup of its own; more than 1 needs the workspace [tokens][kv_heads][parts][2][dim rounded up to a multiple of 32] */
     float *partial;

@@ -211,7 +211,8 @@ __global__ __launch_bounds__(64 * NW, (waves_forward<T, DP, NW>)) void attention
     }
 }
 
-// Backward, first launch: dQ, and delta = rowsum(dO O) for the second.  The forward kernel's shape: dS^T = P^T (dP^T - delta) from S^T = K Q^T and
+// Backward, first launch: dQ, and delta = scale rowsum(dO O) for the second.  dP, delta and so dS carry the scale from the start: rounded to fp16, a large upstream
+// gradient then overflows no sooner than the gradients it leads to.  The forward kernel's shape: dS^T = P^T (dP^T - delta) from S^T = K Q^T and
 // dP^T = V dO^T, then dQ^T = K^T dS^T, K read both ways from one LDS tile.  dQ and dK / dV take a kernel each, which computes S and dP twice (seven
 // products for five), because neither then needs an atomic or a float32 copy of a gradient.
 // A query that sees few keys has gradients that are small differences of dP and delta, and o as it was rounded would set their error.  Where all its keys
@@ -246,7 +247,7 @@ __global__ __launch_bounds__(64 * NW, (waves_dq<T, DP, NW>)) void attention_dq_k
 #pragma unroll
             for (int j = 0; j < 8; ++j) delta += (float)gf[s][j] * (float)of[j];
         }
-        delta += other_half(delta);
+        delta = (delta + other_half(delta)) * p.scale;
     }
     const int64_t at = (int64_t)(w.start + row) * p.heads + head;
     const float lse = row < w.length ? p.lse[at] : 0.f;
@@ -263,7 +264,7 @@ __global__ __launch_bounds__(64 * NW, (waves_dq<T, DP, NW>)) void attention_dq_k
     clear(dq);
     const int last = p.causal ? min(w.length, w.first + BM) - 1 : w.length - 1;
     const int limit = p.causal ? row : w.length - 1;
-    // P and P (dP - delta) of 32 keys
+    // P and scale dP of 32 keys
     auto weights = [&](int n, f32x16 &pr, f32x16 &dp) {
         f32x16 x[2];
         clear(x);
@@ -271,7 +272,7 @@ __global__ __launch_bounds__(64 * NW, (waves_dq<T, DP, NW>)) void attention_dq_k
         mma_rows<T>([&](int y) { return tile::rows(lds_v, 32 * n, y, lane); }, gf, x[1]);
 #pragma unroll
         for (int i = 0; i < 16; ++i) pr[i] = exp2_(x[0][i] * c - mu);
-        dp = x[1];
+        dp = x[1] * p.scale;
     };
     int kt = last / BN;
     const int whole = p.causal ? w.first / BN : w.length / BN;
@@ -340,7 +341,7 @@ __global__ __launch_bounds__(64 * NW, (waves_dq<T, DP, NW>)) void attention_dq_k
         }
     }
     if (row < w.length) {
-        store_row<T>((T *)(p.d_q.p + (int64_t)(w.start + row) * p.d_q.ts + head * p.d_q.hs), dq, p.scale, d, lane);
+        store_row<T>((T *)(p.d_q.p + (int64_t)(w.start + row) * p.d_q.ts + head * p.d_q.hs), dq, 1.f, d, lane);
         if (h == 0) p.delta[at] = delta;
     }
 }
@@ -416,7 +417,7 @@ __global__ __launch_bounds__(64 * NW, (waves_dkv<T, DP>)) void attention_dkv_ker
 #pragma unroll
             for (int j = 0; j < 4; ++j) {
                 x[0][i + j] = exp2_(x[0][i + j] * c - mu[j]);
-                x[1][i + j] = x[0][i + j] * (x[1][i + j] - de[j]);
+                x[1][i + j] = x[0][i + j] * (x[1][i + j] * p.scale - de[j]);
             }
         }
     };
@@ -492,7 +493,7 @@ __global__ __launch_bounds__(64 * NW, (waves_dkv<T, DP>)) void attention_dkv_ker
             store_row<float>(to + DP, dv, 1.f, DP, lane);
         }
     } else if (key < w.length) {
-        store_row<T>((T *)(p.d_k.p + (int64_t)(w.start + key) * p.d_k.ts + kvh * p.d_k.hs), dk, p.scale, d, lane);
+        store_row<T>((T *)(p.d_k.p + (int64_t)(w.start + key) * p.d_k.ts + kvh * p.d_k.hs), dk, 1.f, d, lane);
         store_row<T>((T *)(p.d_v.p + (int64_t)(w.start + key) * p.d_v.ts + kvh * p.d_v.hs), dv, 1.f, d, lane);
     }
 }
@@ -578,7 +579,7 @@ __global__ __launch_bounds__(512, 2) void attention_dkv_pair_kernel(AttentionPar
 #pragma unroll
             for (int j = 0; j < 4; ++j) {
                 x[0][i + j] = exp2_(x[0][i + j] * c - mu[j]);
-                x[1][i + j] = x[0][i + j] * (x[1][i + j] - de[j]);
+                x[1][i + j] = x[0][i + j] * (x[1][i + j] * p.scale - de[j]);
             }
         }
     };
@@ -663,7 +664,7 @@ __global__ __launch_bounds__(512, 2) void attention_dkv_pair_kernel(AttentionPar
         store_row<float>(to, dk, 1.f, DP, lane);
         store_row<float>(to + DP, dv, 1.f, DP, lane);
     } else {
-        store_row<T>((T *)(p.d_k.p + (int64_t)(w.start + key) * p.d_k.ts + kvh * p.d_k.hs), dk, p.scale, d, lane);
+        store_row<T>((T *)(p.d_k.p + (int64_t)(w.start + key) * p.d_k.ts + kvh * p.d_k.hs), dk, 1.f, d, lane);
         store_row<T>((T *)(p.d_v.p + (int64_t)(w.start + key) * p.d_v.ts + kvh * p.d_v.hs), dv, 1.f, d, lane);
     }
 }
@@ -683,7 +684,7 @@ template <typename T, int DP> __global__ __launch_bounds__(256) void attention_s
             dv += *(const f32x4 *)(from + i * 2 * DP + DP);
         }
         if (x < p.dim) {
-            store4((T *)(p.d_k.p + token * p.d_k.ts + kvh * p.d_k.hs) + x, dk[0] * p.scale, dk[1] * p.scale, dk[2] * p.scale, dk[3] * p.scale);
+            store4((T *)(p.d_k.p + token * p.d_k.ts + kvh * p.d_k.hs) + x, dk[0], dk[1], dk[2], dk[3]);
             store4((T *)(p.d_v.p + token * p.d_v.ts + kvh * p.d_v.hs) + x, dv[0], dv[1], dv[2], dv[3]);
         }
     }
@@ -762,7 +763,7 @@ __global__ __launch_bounds__(64, DP == 32 ? 2 : 1) void attention_short_grad_ker
         for (int i = 0; i < 16; ++i) {
             const bool seen = row_of(i, h) <= limit;
             x[0][i] = seen ? exp2_(x[0][i] * c - mu) : 0.f;
-            x[1][i] = seen ? x[1][i] : 0.f;
+            x[1][i] = seen ? x[1][i] * p.scale : 0.f;
             delta += x[0][i] * x[1][i];
         }
         delta += other_half(delta);
@@ -775,7 +776,7 @@ __global__ __launch_bounds__(64, DP == 32 ? 2 : 1) void attention_short_grad_ker
 #pragma unroll
             for (int b = 0; b < DB; ++b) dq[b] += __builtin_nanf("");
         }
-        if (r < length) store_row<T>((T *)(p.d_q.p + (at + r) * p.d_q.ts + head * p.d_q.hs), dq, p.scale, d, lane);
+        if (r < length) store_row<T>((T *)(p.d_q.p + (at + r) * p.d_q.ts + head * p.d_q.hs), dq, 1.f, d, lane);
         // columns: the keys
 #pragma unroll
         for (int y = 0; y < 2; ++y) {
@@ -803,7 +804,7 @@ __global__ __launch_bounds__(64, DP == 32 ? 2 : 1) void attention_short_grad_ker
                 dv[b] += __builtin_nanf("");
             }
         }
-        store_row<T>((T *)(p.d_k.p + (at + r) * p.d_k.ts + kvh * p.d_k.hs), dk, p.scale, d, lane);
+        store_row<T>((T *)(p.d_k.p + (at + r) * p.d_k.ts + kvh * p.d_k.hs), dk, 1.f, d, lane);
         store_row<T>((T *)(p.d_v.p + (at + r) * p.d_v.ts + kvh * p.d_v.hs), dv, 1.f, d, lane);
     }
 }

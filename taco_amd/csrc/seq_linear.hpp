@@ -248,14 +248,15 @@ __global__ __launch_bounds__(STATES ? 2 * DP * (chunk_of<T> / 32) : 4 * DP, 2) v
         return;
     }
     if constexpr (!STATES) {
+        // (the weights carry the scale before they are rounded: in fp16 they overflow no sooner than the outputs they make)
         // decay from key to query inside a block of 32; from an earlier block: the key's to that block's end (to_end), then this lane's query's from there
         float w0[16];
 #pragma unroll
         for (int i = 0; i < 16; ++i) {
             const int n = (lane & 31) - row_of(i, h);
-            w0[i] = n >= 0 ? exp2_(ld * n) : 0.f;
+            w0[i] = n >= 0 ? exp2_(ld * n) * m.scale : 0.f;
         }
-        const float q_entry = exp2_(ld * ((lane & 31) + 1));
+        const float q_entry = exp2_(ld * ((lane & 31) + 1)) * m.scale;
         for (int c0 = 0; c0 < g.count; c0 += C) {
             const int n = advance(c0, []() {});
             const bool bad = nonfinite == c0;
@@ -273,7 +274,7 @@ __global__ __launch_bounds__(STATES ? 2 * DP * (chunk_of<T> / 32) : 4 * DP, 2) v
                 clear(o);
                 // what came before the chunk
                 mma_rows<T>([&](int e) { return tile::rows(lds_s, 32 * slice, e, lane); }, qf, o[0]);
-                o[0] *= exp2_(ld * (32 * qb + (lane & 31) + m.shift));
+                o[0] *= exp2_(ld * (32 * qb + (lane & 31) + m.shift)) * m.scale;
                 // the chunk itself
 #pragma unroll
                 for (int kb = qb; kb >= 0; --kb) {
@@ -303,7 +304,7 @@ __global__ __launch_bounds__(STATES ? 2 * DP * (chunk_of<T> / 32) : 4 * DP, 2) v
 #pragma unroll
                     for (int i = 0; i < 16; i += 4) {
                         const int c = 32 * slice + row_of(i, h);
-                        if (c < d) store4(row + c, o[0][i] * m.scale, o[0][i + 1] * m.scale, o[0][i + 2] * m.scale, o[0][i + 3] * m.scale);
+                        if (c < d) store4(row + c, o[0][i], o[0][i + 1], o[0][i + 2], o[0][i + 3]);
                     }
                 }
             }

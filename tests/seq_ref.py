@@ -47,9 +47,9 @@ def attention(q, k, v, scale, causal, d_o=None, hidden=None):
         o_err = (2 * w[:, None] + (m + 8) * E32) * a_o
         f32 = (2 * w[:, None] + (d + 8) * E32) * a_s + p * (d_o.abs() * o_err).sum(1, keepdim=True)
 
-        def ds_err(u, low):     # P carries the forward's u into o (inside delta), beside o's own rounding; then dS is rounded
+        def ds_err(u, low):     # P carries the forward's u into o (inside delta), beside o's own rounding; then dS is rounded, as scale dS
             o_low = low * (seen @ v.abs() + 1)
-            return f32 + p * (u * delta_abs + (d_o.abs() * (u * a_o + o_low)).sum(1, keepdim=True)) + u * d_s.abs() + low * seen
+            return f32 + p * (u * delta_abs + (d_o.abs() * (u * a_o + o_low)).sum(1, keepdim=True)) + u * d_s.abs() + low / scale * seen
         r.update(dq=scale * d_s @ k, dk=scale * d_s.T @ q, dv=p.T @ d_o)
         r["tol_dq"] = lambda u, low: scale * ds_err(u, low) @ k.abs() + (m + 8) * E32 * scale * a_s @ k.abs() + (u + E32) * r["dq"].abs() + low + 1e-30
         r["tol_dk"] = lambda u, low: scale * ds_err(u, low).T @ q.abs() + (n + 8) * E32 * scale * a_s.T @ q.abs() + (u + E32) * r["dk"].abs() + low + 1e-30
@@ -110,7 +110,7 @@ def linear_bound(name, value, total, n, d, dtype, largest=0.0):
     """Outputs: the weights of a chunk and the state are each rounded to the type for their product (u each, of parts that together make the absolute sum), the output
     once.  States: never rounded.  float32: sums over d, over a chunk's 64 tokens and over the chunks, decays whose exponent (|x| e^-|x| <= 0.4 per step, at
     most two steps each for the chunk, the segment and the whole) is off by a step.  float16: `low` for the up to 64 weights and d state elements of an
-    output, times `largest`, the largest absolute value of what they multiply and of scale."""
+    output, times `largest`, the largest absolute value of what they multiply (the weights carry the scale when they are rounded, the state takes it afterwards)."""
     state = name in ("last", "dstate")
     u, low = (0.0, 0.0) if state else (half_step(dtype), low_step(dtype))
     f32 = E32 * (d + n + 64 + 32)

@@ -394,7 +394,7 @@ def check_linear(lens, H, d, dtype, with_state=True, train=True, decays=None, se
                             g[part].double().cpu() if train else None, d_last[i].double().cpu() if train else None)
         for name, y in got.items():
             mine = y[i] if name in ("last", "dstate") else y[part]
-            near(mine, val[name], R.linear_bound(name, val[name], tot[name], n, d, dtype, abs(sc) * max(float(x.abs().max()) for x in (q, k, v, g))), f"{name}, {dtype}, length {n}, heads {H}, dim {d}")
+            near(mine, val[name], R.linear_bound(name, val[name], tot[name], n, d, dtype, max(1, abs(sc)) * max(float(x.abs().max()) for x in (q, k, v, g))), f"{name}, {dtype}, length {n}, heads {H}, dim {d}")
 
 
 @pytest.mark.parametrize("dtype", DTYPES)
@@ -646,3 +646,17 @@ def test_attention_step_room_past_32_bits():
     got = S().attention_step(q, None, None, kp, vp, wide, n)
     near(got, *want_step(q, [(kp[0, :40].cpu(), vp[0, :40].cpu())], [None], [None], 1 / math.sqrt(d)), "room past 2^31")
     assert (S().attention_step(q, None, None, kp, vp, wide, torch.zeros_like(n)) == 0).all()
+
+
+def test_float16_gradients_that_nearly_fill_its_range():
+    """an upstream gradient of some thousands (a scaled loss): dP is past 65 504, the gradients themselves are not"""
+    d, H, lens = 128, 2, [40, 20]
+    T = sum(lens)
+    q, k, v, g = (randn(T, H, d, dtype=torch.float16, seed=i, scale=s) for i, s in enumerate((0.25, 0.25, 1.0, 4000.0)))
+    q, k, v, g = (x.half() for x in (q, k, v, g))
+    assert torch.isfinite(g).all() and float((g.float()[:, 0] @ v.float()[:, 0].T).abs().max()) > 65504
+    got = run_attention(q, k, v, lens, True, None, g)
+    want = R.attention_heads(*(t.double().cpu() for t in (q, k, v)), lens, 1 / math.sqrt(d), True, torch.float16, g.double().cpu())
+    for name, x in zip(("o", "lse", "dq", "dk", "dv"), got):
+        assert float(want[name][0].abs().max()) < 65504
+        near(x, *want[name], name)
