@@ -351,10 +351,13 @@ __global__ __launch_bounds__(64 * NW, (waves_dq<T, DP, NW>)) void attention_dq_k
 // the lanes; P and dS are the operands of dV^T = dO^T P and dK^T = Q^T dS as they stand.
 // Where the longest sequence's first keys would outlast everything else (all queries of all heads of the group behind one another), the group's heads are
 // shared out to `parts` workgroups, whose float32 sums a third launch adds up, always in the same order (six sequences of up to 4 096: 0.84 -> 0.70 ms + 0.03).
+// Rows of 96 and 128 float32 leave some 150 registers beside the operands and sums: there a tile is 32 queries, Q and dO come in the same registers one after
+// the other, and addresses are computed again for each tile.  100 sequences of up to 200, 8 heads of 128 over 2: 0.20 ms; with tiles of 64 and both at once,
+// which spilled 180 registers, 0.36.
 template <typename T, int DP, int NW>
 __global__ __launch_bounds__(64 * NW, (waves_dkv<T, DP>)) void attention_dkv_kernel(AttentionParams p) {
     typedef Tile<T, DP> tile;
-    constexpr int BK = 32 * NW, BQ = NW == 1 ? 32 : 64, NB = BQ / 32, NS = DP / 16, DB = DP / 32, NT = 64 * NW;
+    constexpr int BK = 32 * NW, BQ = NW == 1 || !ahead<T, DP> ? 32 : 64, NB = BQ / 32, NS = DP / 16, DB = DP / 32, NT = 64 * NW;
     __shared__ __attribute__((aligned(16))) char lds_q[BQ * tile::ROW], lds_g[BQ * tile::ROW];
     __shared__ __attribute__((aligned(16))) float lds_mu[BQ], lds_delta[BQ];
     __shared__ int nonfinite;       // the last query of the tile with something not finite in its row or its gradient's
@@ -383,24 +386,51 @@ __global__ __launch_bounds__(64 * NW, (waves_dkv<T, DP>)) void attention_dkv_ker
     const int whole = p.causal ? min(qt1, (w.first + BK) / BQ) : 0;      // tiles from here on hide no key of the workgroup
     Staged<T, DP, BQ, NT> sq, sg;
     float mu_r = 0.f, delta_r = 0.f;
-    auto fetch = [&](int head, int qt) {
+    auto place = [&]() { return ahead<T, DP> ? t : afresh(t); };      // (wide float32 rows: no register holds an address from tile to tile)
+    auto fetch_q = [&](int head, int qt) {
         const int q0 = qt * BQ, n = min(BQ, w.length - q0);
         const int64_t at = w.start + q0;
-        sq.load(rows_of(p.q.p + at * p.q.ts + head * p.q.hs, n, p.q.ts, rb), p.q.ts, d, t);
-        sg.load(rows_of(p.d_o.p + at * p.d_o.ts + head * p.d_o.hs, n, p.d_o.ts, rb), p.d_o.ts, d, t);
+        sq.load(rows_of(p.q.p + at * p.q.ts + head * p.q.hs, n, p.q.ts, rb), p.q.ts, d, place());
         if (t < BQ) {
             float lse = t < n ? p.lse[(at + t) * p.heads + head] : -__builtin_inff();
             delta_r = t < n ? p.delta[(at + t) * p.heads + head] : 0.f;
             mu_r = lse == -__builtin_inff() ? __builtin_inff() : lse * LOG2E;
         }
     };
-    auto put = [&]() {
-        sq.put(lds_q, t);
-        sg.put(lds_g, t);
+    auto fetch_g = [&](int head, int qt) {
+        const int q0 = qt * BQ, n = min(BQ, w.length - q0);
+        const int64_t at = w.start + q0;
+        sg.load(rows_of(p.d_o.p + at * p.d_o.ts + head * p.d_o.hs, n, p.d_o.ts, rb), p.d_o.ts, d, place());
+    };
+    auto fetch = [&](int head, int qt) {
+        fetch_q(head, qt);
+        fetch_g(head, qt);
+    };
+    auto hide_nonfinite = [&](auto &s) {
+        if (!__any(s.any_nonfinite())) return;
+        int r = -1;
+#pragma unroll
+        for (int i = 0; i < Staged<T, DP, BQ, NT>::N; ++i)
+            if (s.chunk_nonfinite(i)) r = (i * NT + t) / tile::NC;
+        s.nonfinite_to_zero();
+        atomicMax(&nonfinite, r);
+    };
+    auto column = [&]() { return ahead<T, DP> ? lane : afresh(lane); };
+    // the tile to LDS; where nothing travels ahead, Q first and dO after it, in the same registers
+    auto bring = [&](int head, int qt, auto masked) {
+        if (!ahead<T, DP>) fetch_q(head, qt);
+        if (decltype(masked)::value) hide_nonfinite(sq);
+        sq.put(lds_q, place());
         if (t < BQ) {
             lds_mu[t] = mu_r;
             lds_delta[t] = delta_r;
         }
+        if (!ahead<T, DP>) {
+            in_order<T, DP>();
+            fetch_g(head, qt);
+        }
+        if (decltype(masked)::value) hide_nonfinite(sg);
+        sg.put(lds_g, place());
     };
 
     f32x16 dk[DB], dv[DB];
@@ -409,8 +439,8 @@ __global__ __launch_bounds__(64 * NW, (waves_dkv<T, DP>)) void attention_dkv_ker
     // P and dS of 32 queries
     auto weights = [&](int n, f32x16 (&x)[2]) {
         clear(x);
-        mma_rows<T>([&](int y) { return tile::rows(lds_q, 32 * n, y, lane); }, kf, x[0]);
-        mma_rows<T>([&](int y) { return tile::rows(lds_g, 32 * n, y, lane); }, vf, x[1]);
+        mma_rows<T>([&](int y) { return tile::rows(lds_q, 32 * n, y, column()); }, kf, x[0]);
+        mma_rows<T>([&](int y) { return tile::rows(lds_g, 32 * n, y, column()); }, vf, x[1]);
 #pragma unroll
         for (int i = 0; i < 16; i += 4) {
             f32x4 mu = *(const f32x4 *)(lds_mu + 32 * n + row_of(i, h)), de = *(const f32x4 *)(lds_delta + 32 * n + row_of(i, h));
@@ -432,17 +462,7 @@ __global__ __launch_bounds__(64 * NW, (waves_dkv<T, DP>)) void attention_dkv_ker
         };
         for (; qt < whole; ++qt) {
             __syncthreads();
-            if (!ahead<T, DP>) fetch(head, qt);
-            if (__any(sq.any_nonfinite() || sg.any_nonfinite())) {
-                int r = -1;
-#pragma unroll
-                for (int i = 0; i < Staged<T, DP, BQ, NT>::N; ++i)
-                    if (sq.chunk_nonfinite(i) || sg.chunk_nonfinite(i)) r = (i * NT + t) / tile::NC;
-                sq.nonfinite_to_zero();
-                sg.nonfinite_to_zero();
-                atomicMax(&nonfinite, r);
-            }
-            put();
+            bring(head, qt, std::true_type());
             __syncthreads();
             const int seen_bad = nonfinite;
             next();
@@ -458,8 +478,8 @@ __global__ __launch_bounds__(64 * NW, (waves_dkv<T, DP>)) void attention_dkv_ker
                     x[0][i] = seen ? x[0][i] : 0.f;
                     x[1][i] = seen ? x[1][i] : 0.f;
                 }
-                add_columns<T, DP>(lds_g, 32 * n, x[0], dv, lane);
-                add_columns<T, DP>(lds_q, 32 * n, x[1], dk, lane);
+                add_columns<T, DP>(lds_g, 32 * n, x[0], dv, column());
+                add_columns<T, DP>(lds_q, 32 * n, x[1], dk, column());
             }
             if (seen_bad >= 0 && key <= qt * BQ + seen_bad) {       // (a key that such a query sees: its gradients are not finite)
 #pragma unroll
@@ -473,16 +493,15 @@ __global__ __launch_bounds__(64 * NW, (waves_dkv<T, DP>)) void attention_dkv_ker
         }
         for (; qt < qt1; ++qt) {
             __syncthreads();
-            if (!ahead<T, DP>) fetch(head, qt);
-            put();
+            bring(head, qt, std::false_type());
             __syncthreads();
             next();
 #pragma unroll
             for (int n = 0; n < NB; ++n) {
                 f32x16 x[2];
                 weights(n, x);
-                add_columns<T, DP>(lds_g, 32 * n, x[0], dv, lane);
-                add_columns<T, DP>(lds_q, 32 * n, x[1], dk, lane);
+                add_columns<T, DP>(lds_g, 32 * n, x[0], dv, column());
+                add_columns<T, DP>(lds_q, 32 * n, x[1], dk, column());
             }
         }
     }
