@@ -213,7 +213,7 @@ def lists(monkeypatch, lens):
 
 
 @pytest.mark.parametrize("heads", [1, 4, 200])
-@pytest.mark.parametrize("lens", [[1], [0, 5, 0], [64, 65, 128, 129], [1000, 3, 33, 40000], [32] * 500])
+@pytest.mark.parametrize("lens", [[1], [0, 5, 0], [64, 65, 128, 129], [1000, 3, 33, 40000], [32] * 500, [200] * 300 + [0, 32, 33, 64] * 3])
 def test_tiles_cover_every_token_once(monkeypatch, lens, heads):
     seqs = lists(monkeypatch, lens)
     seen = np.zeros(sum(lens), int)

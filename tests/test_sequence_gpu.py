@@ -60,12 +60,14 @@ def test_attention_and_its_gradients(dtype, H, Hk, d, lens):
 
 @pytest.mark.parametrize("dtype", DTYPES)
 @pytest.mark.parametrize("d", [32, 64, 96, 128])
-def test_attention_in_tiles_of_128_rows(dtype, d):
-    """enough tiles that the wide form runs (256 and more, heads counted), with short sequences beside the long ones"""
+@pytest.mark.parametrize("few,launches", [(0, [(128, 6, 0), (32, 3, 1)]), (1024, [(128, 8, 0)])])
+def test_attention_in_tiles_of_128_rows(monkeypatch, dtype, d, few, launches):
+    """enough tiles that the wide form runs (256 and more, heads counted), with short sequences beside the long ones, in tiles of their own and in the same ones"""
+    monkeypatch.setattr(S(), "_FEW_SHORT", few)
     lens = [129, 64, 300, 1, 128]
     check_attention(60, 20, d, lens, dtype)
     seqs = S().Packed(lens, "cuda:0")
-    assert [(x[0], x[3], x[4]) for x in seqs._tiles(60)] == [(128, 6, 0), (32, 3, 1)]
+    assert [(x[0], x[3], x[4]) for x in seqs._tiles(60)] == launches
 
 
 @pytest.mark.parametrize("dtype", DTYPES)
