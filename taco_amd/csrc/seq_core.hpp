@@ -65,6 +65,24 @@ __device__ __forceinline__ float rounded(float x) {
 }
 constexpr float LOG2E = 1.4426950408889634f, LN2 = 0.6931471805599453f;
 
+// ---- float16's range.  An operand that is rounded for a product (a weight, its gradient, a state) may lie outside float16's range, or below 2^-14, where digits are
+// lost, while the inputs and the result do not.  It is multiplied by a power of two first and the product divided by it, both exact.
+template <typename T> constexpr bool narrow = __is_same(T, f16);
+// the power of two that brings the largest absolute value m to [2^14, 2^15); at most 2^64
+__device__ __forceinline__ float lift_of(float m) { return __builtin_bit_cast(float, (268 - max((int)(__builtin_bit_cast(uint32_t, m) >> 23), 77)) << 23); }
+__device__ __forceinline__ float inverse(float power_of_two) { return __builtin_bit_cast(float, (254u << 23) - __builtin_bit_cast(uint32_t, power_of_two)); }
+// The largest value of an operand is between: what is small beside it loses no more than 2^-17 of it (half a step below 2^-14 is 2^-25), less than a half step of the
+// type does, and nothing is lifted.  Nothing but zeros needs no lift either.
+__device__ __forceinline__ bool in_range(float m) { return m == 0.f || (m >= 0.00390625f && m < 32768.f); }
+template <int N> __device__ __forceinline__ float largest(const f32x16 (&x)[N]) {
+    float m[4] = {0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+    for (int n = 0; n < N; ++n)
+#pragma unroll
+        for (int i = 0; i < 16; ++i) m[i % 4] = fmaxf(m[i % 4], __builtin_fabsf(x[n][i]));
+    return fmaxf(fmaxf(m[0], m[1]), fmaxf(m[2], m[3]));
+}
+
 // ---- LDS tiles: rows of DP elements (the head dimension padded with zeros to 32, 64, 96 or 128; 96 in the room of 128), 16-byte chunks exchanged inside each row by an XOR that
 // depends on the row.  256 bytes are one turn of the 64 banks.  A row-wise read (32 rows, the same chunk) wants 16 neighbouring rows in 16 different
 // chunk positions; a column-wise read (4 neighbouring rows, 64 bytes each) wants the four rows in different quarters.  flip() gives both.

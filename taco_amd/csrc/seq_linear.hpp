@@ -91,7 +91,8 @@ template <typename T, int DP, int C> __device__ __forceinline__ void add_outer(c
 // the same number of matrix instructions each: one holds the columns of the state, float32, in registers and updates them (K^T V with the decays); the
 // other makes the outputs from the state before the chunk (P^T = K Q^T with the decays, O^T = V^T P^T + S^T Q^T), which the first leaves for it in LDS as
 // the operand it will be.  One wavefront for both would need more registers than two on a SIMD can have, and then nothing hides its waits.
-// P and S are rounded to the inputs' type for their products, the state itself never is.
+// P and S are rounded to the inputs' type for their products, the state itself never is.  In float16 a column of S that does not fit the type is lifted by a power of two (a
+// gradient's state is divided by the scale: 5 800 is past 65 504 there with heads of 128).
 // 28 700 tokens in 6 sequences, 16 heads of 128, bf16: 0.15 ms for the outputs, 3.1 TB/s (without the outputs' products 0.10: the rest is their latency), 0.07 for
 // the segments' own states, 0.01 for joining them: 0.21 ms in all.  With one wavefront for both parts and its spills it took 0.58.
 // STATES: only the state that the segment makes from nothing, for `carry`; there are fewer of these than CUs, so each chunk is shared out to QB keepers, 32
@@ -103,6 +104,8 @@ __global__ __launch_bounds__(STATES ? 2 * DP * (chunk_of<T> / 32) : 4 * DP, 2) v
     constexpr int C = chunk_of<T>, NT = STATES ? 2 * DP * (C / 32) : 4 * DP, NS = DP / 16, DB = DP / 32, QB = C / 32;
     __shared__ __attribute__((aligned(16))) char lds_k[C * tile::ROW], lds_v[C * tile::ROW], lds_q[STATES ? 16 : C * tile::ROW];
     __shared__ __attribute__((aligned(16))) char lds_s[STATES ? 16 : DP * tile::ROW];      // the state before the chunk, transposed
+    __shared__ __attribute__((aligned(16))) float lowered[narrow<T> && !STATES ? DP : 4];   // what undoes the lift of each column of that state,
+    __shared__ int lifted[DB];                                                              // where a block of 32 columns has one
     __shared__ __attribute__((aligned(16))) float tail[C], to_end[32];      // decay from each token to the last of the chunk; of 32 tokens
     __shared__ int first_bad[DP];
     __shared__ int nonfinite;        // the chunk (its first token) whose V holds something not finite
@@ -184,15 +187,31 @@ __global__ __launch_bounds__(STATES ? 2 * DP * (chunk_of<T> / 32) : 4 * DP, 2) v
             for (int b = 0; b < DB; ++b) s[b] *= f;
         }
         for (int c0 = 0; c0 < g.count; c0 += C) {
+            bool lift = false;
+            float f = 1.f;
+            if constexpr (narrow<T> && !STATES) {
+                float x = largest(s);
+                lift = __any(!in_range(x));
+                if (lift) {
+                    x = fmaxf(x, other_half(x));
+                    f = in_range(x) ? 1.f : lift_of(x);
+                }
+            }
             const int n = advance(c0, [&]() {
                 if constexpr (!STATES) {
+                    auto store = [&](auto g) {
 #pragma unroll
-                    for (int b = 0; b < DB; ++b)
+                        for (int b = 0; b < DB; ++b)
 #pragma unroll
-                        for (int i = 0; i < 16; i += 4) {
-                            const int r = 32 * b + row_of(i, h);
-                            store4((T *)(lds_s + tile::at(col, r / tile::CE) + r % tile::CE * (int)sizeof(T)), s[b][i], s[b][i + 1], s[b][i + 2], s[b][i + 3]);
-                        }
+                            for (int i = 0; i < 16; i += 4) {
+                                const int r = 32 * b + row_of(i, h);
+                                store4((T *)(lds_s + tile::at(col, r / tile::CE) + r % tile::CE * (int)sizeof(T)), g(s[b][i]), g(s[b][i + 1]), g(s[b][i + 2]), g(s[b][i + 3]));
+                            }
+                    };
+                    if (narrow<T> && lift) store([&](float y) { return y * f; });
+                    else store([](float y) { return y; });
+                    if (narrow<T> && lift && h == 0) lowered[col] = inverse(f);
+                    if (narrow<T> && lane == 0) lifted[slice] = lift;
                 }
             });
             // (shift 0: the chunk's own part decays once more, behind its product: a strong decay would leave nothing of it in fp16)
@@ -275,6 +294,14 @@ __global__ __launch_bounds__(STATES ? 2 * DP * (chunk_of<T> / 32) : 4 * DP, 2) v
                 // what came before the chunk
                 mma_rows<T>([&](int e) { return tile::rows(lds_s, 32 * slice, e, lane); }, qf, o[0]);
                 o[0] *= exp2_(ld * (32 * qb + (lane & 31) + m.shift)) * m.scale;
+                if (narrow<T> && lifted[slice]) {
+#pragma unroll
+                    for (int i = 0; i < 16; i += 4) {
+                        const f32x4 u = *(const f32x4 *)(lowered + 32 * slice + row_of(i, h));
+#pragma unroll
+                        for (int j = 0; j < 4; ++j) o[0][i + j] *= u[j];
+                    }
+                }
                 // the chunk itself
 #pragma unroll
                 for (int kb = qb; kb >= 0; --kb) {

@@ -549,8 +549,8 @@ def linear_attention(q, k, v, log_decay, sequences, state=None, scale=None):
     """S_t = exp(log_decay[head]) S_{t-1} + k_t v_t^T, o_t = scale * q_t S_t inside each of `sequences` (a Packed): q, k, v [T, heads, dim], log_decay float32 [heads]
     (<= 0 in earnest; -inf: only the token itself), state float32 [sequences, heads, dim, dim] (key dimension first) or None: the states to begin with.
     scale: 1 / sqrt(dim).  -> (o [T, heads, dim], the states behind the last tokens, float32).  Gradients for q, k, v and state.
-    In float16 the states have to stay inside float16's range (65 504), which their product with q goes through.  A later token has no influence on an
-    earlier output, even where it holds NaN or infinities; a value that is not finite makes the outputs of its own chunk of 64 tokens and the state NaN."""
+    A later token has no influence on an earlier output, even where it holds NaN or infinities; a value that is not finite makes the outputs of its own chunk of
+    64 tokens and the state NaN.  In float16 a growth (log_decay > 0) must leave v exp(64 log_decay) inside the type's range."""
     device, _ = _check_rows("linear_attention", q, ("k", k), ("v", v))
     if not q.shape == k.shape == v.shape or not q.shape[1]:
         raise ValueError(f"q {tuple(q.shape)}, k {tuple(k.shape)}, v {tuple(v.shape)}: alike expected")

@@ -1,0 +1,59 @@
+"""float16's range inside the sequence kernels: what they round for their matrix products (weights, their gradients, states) keeps its digits, and stays finite, wherever the
+inputs and the results fit the type."""
+import math
+
+import pytest
+import torch
+
+import seq_ref as R
+from test_sequence_gpu import S, near, randn
+
+pytestmark = pytest.mark.gpu
+F16 = torch.float16
+
+
+def linear_case(lens, d, seed=0, heads=2, q=1.0, k=1.0, v=1.0, d_o=1.0, state=1.0, d_last=1.0, scale=None):
+    """-> {name: (kernel's, definition's, absolute sums)} of linear_attention in float16, packed; and the definition's largest output"""
+    T = sum(lens)
+    x = [randn(T, heads, d, dtype=F16, seed=seed + i, scale=s).requires_grad_() for i, s in enumerate((q, k, v))]
+    g = randn(T, heads, d, dtype=F16, seed=seed + 3, scale=d_o)
+    x.append(randn(len(lens), heads, d, d, seed=seed + 4, scale=state).requires_grad_())
+    gs = randn(len(lens), heads, d, d, seed=seed + 5, scale=d_last)
+    decay = torch.tensor([math.log(1 - 0.5 ** (3 + h)) for h in range(heads)], dtype=torch.float32, device="cuda")
+    o, last = S().linear_attention(*x[:3], decay, S().Packed(lens, "cuda:0"), state=x[3], scale=scale)
+    got = dict(zip(("o", "last", "dq", "dk", "dv", "dstate"), (o, last) + torch.autograd.grad((o, last), x, (g, gs))))
+    at, parts = 0, []
+    for i, n in enumerate(lens):
+        part = slice(at, at + n)
+        at += n
+        parts.append(R.linear(*(t[part].detach().double().cpu() for t in x[:3]), decay.double().cpu(), x[3][i].detach().double().cpu(), 1 / math.sqrt(d) if scale is None else scale,
+                              g[part].double().cpu(), gs[i].double().cpu()))
+    rows = [t.detach().abs().amax(-1) for t in x[:3] + [g]]
+    out = {"n": max(lens), "spread": max(float(r.max() / r.min()) for r in rows)}
+    for name, t in got.items():
+        join = torch.stack if name in ("last", "dstate") else torch.cat
+        out[name] = (t.detach().double().cpu(),) + tuple(join([p[j][name] for p in parts]) for j in (0, 1))
+    return out
+
+
+def check_linear(out, d):
+    """Within the roundings that the operator states, none of which falls below the type's normal range: seq_ref's bound without what that would add (`largest` 0), and for what
+    the kernels do not lift, a weight (state) of at least 2^-8 with smaller ones beside it: those are off by half of float16's smallest step, 2^-25, so 2^-17 of the
+    largest, up to 64 weights and d elements of an output, times what they multiply.  The largest product of the two is at most the largest absolute sum times
+    the ratio `spread` between the largest element of a tensor and the largest of any row."""
+    spread, n = out.pop("spread"), out.pop("n")
+    for name, (got, value, total) in out.items():
+        state = name in ("last", "dstate")
+        assert state or 0.01 < float(value.abs().max()) < 65504, name
+        near(got, value, R.linear_bound(name, value, total, n, d, F16) + (0 if state else 2.0 ** -17 * (64 + d) * spread * float(total.max())), name)
+
+
+@pytest.mark.parametrize("lens", [[40, 1, 130], [600, 300]])
+@pytest.mark.parametrize("d,kw", [
+    (128, dict(d_last=2000.0, v=0.1, k=0.1)),                       # (d_last / scale is past 65 504)
+    (64, dict(d_last=100.0, scale=1e-3)),
+    (80, dict(d_last=5.0, scale=1.0 / 4096, d_o=50.0)),
+    (128, dict(state=60000.0, q=0.005, d_o=0.1))])
+def test_linear_attention_states_past_float16(lens, d, kw):
+    """states, and state gradients over the scale, past float16's range where their products with q, k and v are not"""
+    check_linear(linear_case(lens, d, **kw), d)
