@@ -267,7 +267,7 @@ __global__ __launch_bounds__(STATES ? 2 * DP * (chunk_of<T> / 32) : 4 * DP, 2) v
         return;
     }
     if constexpr (!STATES) {
-        // (the weights carry the scale before they are rounded: in fp16 they overflow no sooner than the outputs they make)
+        // (the weights carry the scale before they are rounded; in float16, those of a block and query that do not fit the type are lifted by a power of two)
         // decay from key to query inside a block of 32; from an earlier block: the key's to that block's end (to_end), then this lane's query's from there
         float w0[16];
 #pragma unroll
@@ -317,8 +317,21 @@ __global__ __launch_bounds__(STATES ? 2 * DP * (chunk_of<T> / 32) : 4 * DP, 2) v
                         for (int j = 0; j < 4; ++j)
                             x[0][i + j] = kb == qb ? ((lane & 31) >= row_of(i + j, h) ? x[0][i + j] * w0[i + j] : 0.f) : x[0][i + j] * (w[j] * q_entry);
                     }
+                    float f = 1.f;          // (outside: the whole sum is lifted with this block's weights, and lowered behind them)
+                    bool lift = false;
+                    if constexpr (narrow<T>) {
+                        float y = largest(x);
+                        lift = __any(!in_range(y));
+                        if (lift) {
+                            y = fmaxf(y, other_half(y));
+                            f = in_range(y) ? 1.f : lift_of(y);
+                            x[0] *= f;
+                            o[0] *= f;
+                        }
+                    }
 #pragma unroll
                     for (int e = 0; e < 2; ++e) o[0] = mma(vf[e], to_frag<T>(x[0], e), o[0]);
+                    if (narrow<T> && lift) o[0] *= inverse(f);
                 }
                 if (bad) {
 #pragma unroll

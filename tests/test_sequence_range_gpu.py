@@ -48,6 +48,15 @@ def check_linear(out, d):
         near(got, value, R.linear_bound(name, value, total, n, d, F16) + (0 if state else 2.0 ** -17 * (64 + d) * spread * float(total.max())), name)
 
 
+def check_rms(got, value, times, what):
+    """root mean square errors: at most `times` that of the value rounded once"""
+    got, value = got.detach().double().cpu(), value.double()
+    assert torch.isfinite(got).all(), what
+    once = float((value.half().double() - value).square().mean().sqrt())
+    err = float((got - value).square().mean().sqrt())
+    assert err <= times * once, f"{what}: {err:.3g}, {err / once:.3g} x the value rounded once"
+
+
 @pytest.mark.parametrize("lens", [[40, 1, 130], [600, 300]])
 @pytest.mark.parametrize("d,kw", [
     (128, dict(d_last=2000.0, v=0.1, k=0.1)),                       # (d_last / scale is past 65 504)
@@ -57,3 +66,22 @@ def check_linear(out, d):
 def test_linear_attention_states_past_float16(lens, d, kw):
     """states, and state gradients over the scale, past float16's range where their products with q, k and v are not"""
     check_linear(linear_case(lens, d, **kw), d)
+
+
+@pytest.mark.parametrize("lens", [[40, 1, 130], [600, 300]])
+def test_linear_attention_weights_past_float16(lens):
+    """weights past 65 504 whose outputs are not: large q and k with small v, and the same of d_o and v with small k and q"""
+    check_linear(linear_case(lens, 64, q=160.0, k=2000.0, v=1e-3, d_o=1e-3, state=1.0, d_last=1e-3, scale=1.0), 64)
+    check_linear(linear_case(lens, 64, q=0.005, k=0.005, v=60.0, d_o=8000.0, state=1.0, d_last=1.0), 64)
+
+
+@pytest.mark.parametrize("kw", [dict(d_o=1e-3, v=0.02, k=30.0, q=30.0, state=0.02, d_last=1e-3), dict(v=2e-4, k=0.05, q=30.0, state=1e-5, d_last=0.01, d_o=30.0)])
+def test_linear_attention_small_weights(kw):
+    """Weights and states below float16's normal range with results inside it.  Three roundings of a size (a weight, a state, the output), independent: sqrt(3) times the error of
+    one, and three leaves room for their being unequal."""
+    lens, d = [300, 700], 64
+    out = linear_case(lens, d, **kw)
+    for name in ("o", "dq", "dk", "dv"):
+        got, value, _ = out[name]
+        assert float(value.abs().median()) > 2.0 ** -13, name
+        check_rms(got, value, 3, name)
