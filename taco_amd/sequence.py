@@ -11,7 +11,8 @@ row and call).  The reference's policies remember through frame stacks and an LS
     out = sequence.linear_attention_step(q, k, v, log_decay, state, reset=env.reset_buf)
 
 float32, float16 and bfloat16; head dimensions that are multiples of 8 up to 128; sums, softmax statistics and states are float32.  Work is enqueued on the
-current stream of the tensors' device, nothing synchronises, and every call gives the same bits each time.  There is no torch fallback.
+current stream of the tensors' device, nothing synchronises, and every call gives the same bits each time.  There is no torch fallback, no forward-mode derivative
+and no second derivative: what asks for one is refused.
 
 HIP graphs: call once eagerly before capturing (the work lists are uploaded at the first call with a given number of heads), keep the Packed alive as long as
 the graph, and capture a backward pass only while no eager autograd graph of the same leaf tensors is alive: torch then waits for the eager graph's stream
@@ -22,6 +23,7 @@ import math
 
 import numpy as np
 import torch
+from torch.autograd import forward_ad
 
 from . import _lib
 
@@ -163,6 +165,10 @@ def _check_out(out, q):
 def _scale(scale, dim, positive):
     if scale is None:
         return 1.0 / math.sqrt(dim)
+    if isinstance(scale, torch.Tensor):
+        _no_tangent("the scale", scale)
+        if scale.requires_grad and torch.is_grad_enabled():
+            raise _lib.TacoError("the scale has no gradient: give its value, or multiply q by it")
     scale = float(scale)
     if not math.isfinite(scale) or scale == 0 or (positive and scale < 0):
         raise ValueError(f"scale {scale}: {'positive and finite' if positive else 'finite and not 0'}")
@@ -172,6 +178,12 @@ def _scale(scale, dim, positive):
 def _no_grad(tensors, what):
     if torch.is_grad_enabled() and any(t is not None and t.requires_grad for t in tensors):
         raise _lib.TacoError(f"{what} has no gradient: call it under torch.no_grad(), or use the form over whole sequences")
+
+
+def _no_tangent(what, *tensors):
+    """a dual tensor does not require a gradient: without this its tangent would be lost, and the result count as constant"""
+    if forward_ad._current_level >= 0 and any(t is not None and forward_ad.unpack_dual(t).tangent is not None for t in tensors):
+        raise _lib.TacoError(f"{what} has no forward-mode derivative")
 
 
 def _check_packed(seqs, device, rows):
@@ -378,6 +390,7 @@ def attention(q, k, v, sequences, causal=True, scale=None, return_lse=False, out
     A token that is hidden has no influence, even where it holds NaN or infinities, forward and backward; a token whose scores are all -inf gets zeros.  Rows behind the last sequence: zero in new
     tensors and in gradients, untouched in `out` (which cannot be given where a gradient is recorded, and must not overlap q, k or v).
     Strides: any, as long as `dim` is contiguous and rows are multiples of 16 bytes; other layouts are copied first."""
+    _no_tangent("attention", q, k, v, out)
     device, _ = _check_rows("attention", q, ("k", k), ("v", v))
     (T, H, d), Hk = q.shape, k.shape[1]
     if k.shape != v.shape or k.shape[0] != T:
@@ -424,6 +437,7 @@ def attention_step(q, k, v, k_pages, v_pages, page_table, lengths, scale=None, o
     gives NaN; nothing else is touched.  -> [rows, heads, dim] (`out` if given, which must not overlap the inputs).  No gradient."""
     if (k is None) != (v is None):
         raise ValueError("k and v: both or none")
+    _no_tangent("attention_step", q, k, v, k_pages, v_pages, out)
     device, code = _check_rows("attention_step", q) if k is None else _check_rows("attention_step", q, ("k", k), ("v", v))
     B, H, d = q.shape
     ks, vs = _check_pages("k_pages", k_pages, q), _check_pages("v_pages", v_pages, q)
@@ -551,6 +565,7 @@ def linear_attention(q, k, v, log_decay, sequences, state=None, scale=None):
     scale: 1 / sqrt(dim).  -> (o [T, heads, dim], the states behind the last tokens, float32).  Gradients for q, k, v and state.
     A later token has no influence on an earlier output, even where it holds NaN or infinities; a value that is not finite makes the outputs of its own chunk of
     64 tokens and the state NaN.  In float16 a growth (log_decay > 0) must leave v exp(64 log_decay) inside the type's range."""
+    _no_tangent("linear_attention", q, k, v, log_decay, state)
     device, _ = _check_rows("linear_attention", q, ("k", k), ("v", v))
     if not q.shape == k.shape == v.shape or not q.shape[1]:
         raise ValueError(f"q {tuple(q.shape)}, k {tuple(k.shape)}, v {tuple(v.shape)}: alike expected")
@@ -574,6 +589,7 @@ def linear_attention_step(q, k, v, log_decay, state, reset=None, scale=None, out
     """One token per row of linear_attention: q, k, v [rows, heads, dim]; state float32 [rows, heads, dim, dim], contiguous, updated in place; reset [rows] (bool,
     uint8, int32 or int64, e.g. env.reset_buf): rows that begin anew, whatever their state holds.  -> [rows, heads, dim] (`out` if given, which must not
     overlap the inputs).  No gradient."""
+    _no_tangent("linear_attention_step", q, k, v, log_decay, state, out)
     device, code = _check_rows("linear_attention_step", q, ("k", k), ("v", v))
     shape = q.shape
     B, H, d = shape

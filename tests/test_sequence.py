@@ -287,3 +287,31 @@ int main() {
     exe = str(tmp_path / "t")
     subprocess.check_call(["g++", "-std=c++17", "-O1", "-g", "-fsanitize=address,undefined", "-I", os.path.join(ROOT, "taco_amd", "csrc"), "-o", exe, str(src)])
     assert subprocess.check_output([exe]).strip() == b"ok"
+
+
+def test_tangents_and_scales_that_want_a_gradient_are_refused():
+    """neither requires a gradient of the operands, and neither may be dropped without a word"""
+    s = sequence
+    x, other = torch.zeros(4, 2, 32), [torch.zeros(n) for n in ((6, 16, 2, 32), (6, 16, 2, 32))]
+    table, lens, decay, state = torch.zeros(4, 3, dtype=torch.int32), torch.zeros(4, dtype=torch.int32), torch.zeros(2), torch.zeros(4, 2, 32, 32)
+    seqs = s.Packed([1] * 4, "cuda:0")
+    calls = [(lambda q, k, v, o: s.attention(q, k, v, seqs, out=o), [x, x, x, x]),
+             (lambda q, k, v, a, b, o: s.attention_step(q, k, v, a, b, table, lens, out=o), [x, x, x] + other + [x]),
+             (lambda q, k, v, g, t: s.linear_attention(q, k, v, g, seqs, state=t), [x, x, x, decay, state]),
+             (lambda q, k, v, g, t, o: s.linear_attention_step(q, k, v, g, t, out=o), [x, x, x, decay, state, x])]
+    with torch.autograd.forward_ad.dual_level():
+        for f, args in calls:
+            for i in range(len(args)):
+                with pytest.raises(_lib.TacoError, match="forward-mode"):
+                    f(*args[:i], torch.autograd.forward_ad.make_dual(args[i], torch.ones_like(args[i])), *args[i + 1:])
+            with pytest.raises(_lib.TacoError, match="MI355X"):     # (nothing else is refused for being called here)
+                f(*args)
+        scale = torch.tensor(0.5)
+        with pytest.raises(_lib.TacoError, match="forward-mode"):
+            s._scale(torch.autograd.forward_ad.make_dual(scale, torch.ones(())), 32, True)
+    q = Fake((4, 2, 32))
+    for f in (lambda c: s.attention(q, q, q, seqs, scale=c), lambda c: s.linear_attention(q, q, q, Fake((2,)), seqs, scale=c)):
+        with pytest.raises(_lib.TacoError, match="scale has no gradient"):
+            f(torch.tensor(0.5, requires_grad=True))
+    with torch.no_grad():
+        assert s._scale(torch.tensor(0.5, requires_grad=True), 32, True) == 0.5
