@@ -211,8 +211,9 @@ __global__ __launch_bounds__(64 * NW, (waves_forward<T, DP, NW>)) void attention
     }
 }
 
-// Backward, first launch: dQ, and delta = scale rowsum(dO O) for the second.  dP, delta and so dS carry the scale from the start: rounded to fp16, a large upstream
-// gradient then overflows no sooner than the gradients it leads to.  The forward kernel's shape: dS^T = P^T (dP^T - delta) from S^T = K Q^T and
+// Backward, first launch: dQ, and delta = scale rowsum(dO O) for the second.  dP, delta and so dS carry the scale from the start.  In float16 dS, a product of a weight (of
+// 1 / length), an upstream gradient and the scale, is lifted by a power of two for each query (here) or key (dK) before it is rounded: without, an upstream
+// gradient of a thousandth over 2 048 tokens left dq and dk 25 times as far off as a value rounded once.  The forward kernel's shape: dS^T = P^T (dP^T - delta) from S^T = K Q^T and
 // dP^T = V dO^T, then dQ^T = K^T dS^T, K read both ways from one LDS tile.  dQ and dK / dV take a kernel each, which computes S and dP twice (seven
 // products for five), because neither then needs an atomic or a float32 copy of a gradient.
 // A query that sees few keys has gradients that are small differences of dP and delta, and o as it was rounded would set their error.  Where all its keys
@@ -262,6 +263,7 @@ __global__ __launch_bounds__(64 * NW, (waves_dq<T, DP, NW>)) void attention_dq_k
 
     f32x16 dq[DB];
     clear(dq);
+    float f = lift_start<T>;
     const int last = p.causal ? min(w.length, w.first + BM) - 1 : w.length - 1;
     const int limit = p.causal ? row : w.length - 1;
     // P and scale dP of 32 keys
@@ -312,6 +314,7 @@ __global__ __launch_bounds__(64 * NW, (waves_dq<T, DP, NW>)) void attention_dq_k
                 weights(n, pr, ds);
 #pragma unroll
                 for (int i = 0; i < 16; ++i) ds[i] = k0 + 32 * n + row_of(i, h) <= limit ? pr[i] * (ds[i] - delta) : 0.f;
+                lift<T>(ds, f, dq);
                 add_columns<T, DP>(lds_k, 32 * n, ds, dq, lane);
             }
             if (k0 + seen_bad <= limit && seen_bad < BN) {      // (a key that is not finite: its weight is not either)
@@ -337,11 +340,12 @@ __global__ __launch_bounds__(64 * NW, (waves_dq<T, DP, NW>)) void attention_dq_k
             weights(n, pr, ds);
 #pragma unroll
             for (int i = 0; i < 16; ++i) ds[i] = pr[i] * (ds[i] - delta);
+            lift<T>(ds, f, dq);
             add_columns<T, DP>(lds_k, 32 * n, ds, dq, lane);
         }
     }
     if (row < w.length) {
-        store_row<T>((T *)(p.d_q.p + (int64_t)(w.start + row) * p.d_q.ts + head * p.d_q.hs), dq, 1.f, d, lane);
+        store_row<T>((T *)(p.d_q.p + (int64_t)(w.start + row) * p.d_q.ts + head * p.d_q.hs), dq, inverse(f), d, lane);
         if (h == 0) p.delta[at] = delta;
     }
 }
@@ -436,6 +440,7 @@ __global__ __launch_bounds__(64 * NW, (waves_dkv<T, DP>)) void attention_dkv_ker
     f32x16 dk[DB], dv[DB];
     clear(dk);
     clear(dv);
+    float f = lift_start<T>;
     // P and dS of 32 queries
     auto weights = [&](int n, f32x16 (&x)[2]) {
         clear(x);
@@ -478,6 +483,7 @@ __global__ __launch_bounds__(64 * NW, (waves_dkv<T, DP>)) void attention_dkv_ker
                     x[0][i] = seen ? x[0][i] : 0.f;
                     x[1][i] = seen ? x[1][i] : 0.f;
                 }
+                lift<T>(x[1], f, dk);
                 add_columns<T, DP>(lds_g, 32 * n, x[0], dv, column());
                 add_columns<T, DP>(lds_q, 32 * n, x[1], dk, column());
             }
@@ -500,10 +506,15 @@ __global__ __launch_bounds__(64 * NW, (waves_dkv<T, DP>)) void attention_dkv_ker
             for (int n = 0; n < NB; ++n) {
                 f32x16 x[2];
                 weights(n, x);
+                lift<T>(x[1], f, dk);
                 add_columns<T, DP>(lds_g, 32 * n, x[0], dv, column());
                 add_columns<T, DP>(lds_q, 32 * n, x[1], dk, column());
             }
         }
+    }
+    if constexpr (narrow<T>) {
+#pragma unroll
+        for (int b = 0; b < DB; ++b) dk[b] *= inverse(f);
     }
     if (NW == 4 && p.parts > 1) {
         float *to = p.partial + (((int64_t)(w.start + key) * p.kv_heads + kvh) * p.parts + part) * 2 * DP;
@@ -575,6 +586,7 @@ __global__ __launch_bounds__(512, 2) void attention_dkv_pair_kernel(AttentionPar
     f32x16 dk[DB], dv[DB];
     clear(dk);
     clear(dv);
+    float f = lift_start<T>;
     // P and dS of this wavefront's 32 queries
     auto weights = [&](f32x16 (&x)[2]) {
         clear(x);
@@ -634,6 +646,7 @@ __global__ __launch_bounds__(512, 2) void attention_dkv_pair_kernel(AttentionPar
                     x[0][i] = seen ? x[0][i] : 0.f;
                     x[1][i] = seen ? x[1][i] : 0.f;
                 }
+                lift<T>(x[1], f, dk);
                 add_columns<T, DP>(lds_g, 32 * half, x[0], dv, lane);
                 add_columns<T, DP>(lds_q, 32 * half, x[1], dk, lane);
             }
@@ -654,6 +667,7 @@ __global__ __launch_bounds__(512, 2) void attention_dkv_pair_kernel(AttentionPar
             next();
             f32x16 x[2];
             weights(x);
+            lift<T>(x[1], f, dk);
             add_columns<T, DP>(lds_g, 32 * half, x[0], dv, lane);
             add_columns<T, DP>(lds_q, 32 * half, x[1], dk, lane);
         }
@@ -675,6 +689,10 @@ __global__ __launch_bounds__(512, 2) void attention_dkv_pair_kernel(AttentionPar
                 for (int i = 0; i < 16; ++i) x[b][i] += mine[(b * 16 + i) * 64];
         }
     };
+    if constexpr (narrow<T>) {      // (each of the two wavefronts has a lift of its own)
+#pragma unroll
+        for (int b = 0; b < DB; ++b) dk[b] *= inverse(f);
+    }
     join(dk);
     join(dv);
     if (half || key >= w.length) return;
@@ -719,8 +737,9 @@ template <typename T, int DP>
 __global__ __launch_bounds__(64, DP == 32 ? 2 : 1) void attention_short_grad_kernel(AttentionParams p) {
     typedef Tile<T, DP> tile;
     typedef Tile<T, 32> square;
+    typedef Tile<float, 32> square32;       // dS in float16: lifted by key, once it is turned
     constexpr int NS = DP / 16, DB = DP / 32;
-    __shared__ __attribute__((aligned(16))) char lds_k[32 * tile::ROW], lds_q[32 * tile::ROW], lds_g[32 * tile::ROW], lds_w[32 * square::ROW];
+    __shared__ __attribute__((aligned(16))) char lds_k[32 * tile::ROW], lds_q[32 * tile::ROW], lds_g[32 * tile::ROW], lds_w[32 * (narrow<T> ? square32::ROW : square::ROW)];
     int ti, kvh;
     locate(blockIdx.x, p.kv_heads, ti, kvh);
     const taco_seq_tile w = p.key_tiles[ti];
@@ -759,6 +778,7 @@ __global__ __launch_bounds__(64, DP == 32 ? 2 : 1) void attention_short_grad_ker
     f32x16 dk[DB], dv[DB];
     clear(dk);
     clear(dv);
+    float fk = lift_start<T>;
     int bad_query = -1;
     for (int head = kvh * G; head < (kvh + 1) * G; ++head) {
         const rsrc rq = rows_of(p.q.p + at * p.q.ts + head * p.q.hs, length, p.q.ts, rb), rg = rows_of(p.d_o.p + at * p.d_o.ts + head * p.d_o.hs, length, p.d_o.ts, rb);
@@ -790,22 +810,40 @@ __global__ __launch_bounds__(64, DP == 32 ? 2 : 1) void attention_short_grad_ker
         for (int i = 0; i < 16; ++i) x[1][i] = row_of(i, h) <= limit ? x[0][i] * (x[1][i] - delta) : 0.f;
         f32x16 dq[DB];
         clear(dq);
+        float fq = lift_start<T>;
+        lift<T>(x[1], fq, dq);
         add_columns<T, DP>(lds_k, 0, x[1], dq, lane);
         if (bad_key <= limit) {
 #pragma unroll
             for (int b = 0; b < DB; ++b) dq[b] += __builtin_nanf("");
         }
-        if (r < length) store_row<T>((T *)(p.d_q.p + (at + r) * p.d_q.ts + head * p.d_q.hs), dq, 1.f, d, lane);
+        if (r < length) store_row<T>((T *)(p.d_q.p + (at + r) * p.d_q.ts + head * p.d_q.hs), dq, inverse(fq), d, lane);
         // columns: the keys
 #pragma unroll
         for (int y = 0; y < 2; ++y) {
             __syncthreads();
-#pragma unroll
-            for (int i = 0; i < 16; ++i) *(T *)(lds_w + square::at(row_of(i, h), r / square::CE) + r % square::CE * (int)sizeof(T)) = (T)x[y][i];
-            __syncthreads();
             frag<T> f[2];
+            if (narrow<T> && y == 1) {
 #pragma unroll
-            for (int s = 0; s < 2; ++s) f[s] = square::rows_permuted(lds_w, 0, 16 * s, lane);
+                for (int i = 0; i < 16; ++i) *(float *)(lds_w + square32::at(row_of(i, h), r / 4) + r % 4 * 4) = x[1][i] * inverse(fq);
+                __syncthreads();
+                f32x16 z;
+#pragma unroll
+                for (int s = 0; s < 2; ++s) {
+                    const f32x8 a = square32::rows_permuted(lds_w, 0, 16 * s, lane);
+#pragma unroll
+                    for (int j = 0; j < 8; ++j) z[8 * s + j] = a[j];
+                }
+                lift<T>(z, fk, dk);
+#pragma unroll
+                for (int s = 0; s < 2; ++s) f[s] = to_frag<T>(z, s);
+            } else {
+#pragma unroll
+                for (int i = 0; i < 16; ++i) *(T *)(lds_w + square::at(row_of(i, h), r / square::CE) + r % square::CE * (int)sizeof(T)) = (T)x[y][i];
+                __syncthreads();
+#pragma unroll
+                for (int s = 0; s < 2; ++s) f[s] = square::rows_permuted(lds_w, 0, 16 * s, lane);
+            }
 #pragma unroll
             for (int s = 0; s < 2; ++s)
 #pragma unroll
@@ -814,6 +852,10 @@ __global__ __launch_bounds__(64, DP == 32 ? 2 : 1) void attention_short_grad_ker
                     else dk[b] = mma(tile::cols(lds_q, 16 * s, 32 * b, lane), f[s], dk[b]);
                 }
         }
+    }
+    if constexpr (narrow<T>) {
+#pragma unroll
+        for (int b = 0; b < DB; ++b) dk[b] *= inverse(fk);
     }
     if (r < length) {
         if (r <= bad_query) {       // (a key that such a query sees: its gradients are not finite)

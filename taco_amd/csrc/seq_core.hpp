@@ -82,6 +82,23 @@ template <int N> __device__ __forceinline__ float largest(const f32x16 (&x)[N]) 
         for (int i = 0; i < 16; ++i) m[i % 4] = fmaxf(m[i % 4], __builtin_fabsf(x[n][i]));
     return fmaxf(fmaxf(m[0], m[1]), fmaxf(m[2], m[3]));
 }
+// An operand that is made block by block while a product runs, a column (lane) at a time: x becomes x times a power of two `f` that the column keeps, chosen by its largest
+// value so far, and the sums acc with it.  f starts at 2^64 and falls: what comes later and is smaller loses no more than 2^-39 of the largest.
+template <typename T, int N> __device__ __forceinline__ void lift(f32x16 &x, float &f, f32x16 (&acc)[N]) {
+    if constexpr (narrow<T>) {
+        const f32x16 y[1] = {x};
+        float m = largest(y);
+        if (__any(m * f >= 32768.f)) {
+            m = fmaxf(m, other_half(m));
+            const float g = m * f >= 32768.f ? lift_of(m) : f, a = g * inverse(f);
+            f = g;
+#pragma unroll
+            for (int n = 0; n < N; ++n) acc[n] *= a;
+        }
+        x *= f;
+    }
+}
+template <typename T> constexpr float lift_start = narrow<T> ? 18446744073709551616.f : 1.f;
 
 // ---- LDS tiles: rows of DP elements (the head dimension padded with zeros to 32, 64, 96 or 128; 96 in the room of 128), 16-byte chunks exchanged inside each row by an XOR that
 // depends on the row.  256 bytes are one turn of the 64 banks.  A row-wise read (32 rows, the same chunk) wants 16 neighbouring rows in 16 different

@@ -85,3 +85,30 @@ def test_linear_attention_small_weights(kw):
         got, value, _ = out[name]
         assert float(value.abs().median()) > 2.0 ** -13, name
         check_rms(got, value, 3, name)
+
+
+def attention_case(H, n, d, d_o, sink=0.0, seed=0):
+    """one causal sequence, all gradients.  `sink`: the first key gets that much more score from every query, and its value is zero."""
+    q, k, v = (randn(n, H, d, dtype=F16, seed=seed + i) for i in range(3))
+    g = randn(n, H, d, dtype=F16, seed=seed + 3, scale=d_o)
+    if sink:
+        q[:, :, 0], k[:, :, 0], k[0, :, 0], v[0] = 4.0, 0.0, sink * math.sqrt(d) / 4, 0.0
+    x = [t.requires_grad_() for t in (q, k, v)]
+    o = S().attention(*x, S().Packed([n], "cuda:0"))
+    got = (o,) + torch.autograd.grad(o, x, g)
+    want = [[] for _ in got]
+    for h in range(H):
+        r = R.attention(*(t[:, h].detach().double().cpu() for t in x), 1 / math.sqrt(d), True, g[:, h].double().cpu())
+        for w, name in zip(want, ("o", "dq", "dk", "dv")):
+            w.append(r[name])
+    return {name: (a, torch.stack(w, 1)) for name, a, w in zip(("o", "dq", "dk", "dv"), got, want)}
+
+
+# Roundings on the way: the weight P for o, o for delta, the weight's gradient dS, the result; independent and of a size, so twice the error of one, and three leaves
+# room for their being unequal.
+@pytest.mark.parametrize("H,n,d,d_o", [(2, 30, 64, 1e-4), (2, 200, 64, 1e-3), (1, 2048, 64, 1e-3), (1, 1500, 128, 1e-2), (64, 600, 128, 1e-3), (64, 600, 32, 1e-3)])
+def test_attention_small_gradients(H, n, d, d_o):
+    """an upstream gradient of a thousandth (a mean loss): dS, that times the weight and the scale, is far below float16's normal range, dq and dk are not"""
+    for name, (got, want) in attention_case(H, n, d, d_o).items():
+        assert float(want[1:].abs().median()) > 2.0 ** -17, name
+        check_rms(got[1:], want[1:], 3, name)          # (the first query sees one key: its dq is 0)
