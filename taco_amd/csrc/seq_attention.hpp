@@ -42,10 +42,10 @@ template <typename T, int DP> __device__ __forceinline__ void in_order() {
 
 // acc += X w for a product whose tile X of 32 rows is read by columns: one step of a running sum in acc.  float32 sums each tile apart first: the sum over a long
 // sequence then has a rounding per tile in it, not per pair of rows (its error is the float32 result's own; the 16-bit types' roundings are larger).
-template <typename T, int DP> __device__ __forceinline__ void add_columns(const char *lds, int row0, const f32x16 &w, f32x16 (&acc)[DP / 32], int lane) {
+template <typename T, int DP> __device__ __forceinline__ void add_columns(const char *lds, int row0, const f32x16 &w, f32x16 (&acc)[DP / 32], int lane, float factor = 1.f) {
     frag<T> f[2];
 #pragma unroll
-    for (int x = 0; x < 2; ++x) f[x] = to_frag<T>(w, x);
+    for (int x = 0; x < 2; ++x) f[x] = to_frag<T>(w * factor, x);
     if constexpr (sizeof(T) == 4) {
 #pragma unroll
         for (int b = 0; b < DP / 32; ++b) {
@@ -67,7 +67,8 @@ template <typename T, int DP> __device__ __forceinline__ void add_columns(const 
 // Forward.  A wavefront owns 32 queries (columns of all its products), a workgroup NW of them and one K and one V tile of BN keys in LDS; the next tiles travel
 // in registers meanwhile.  S^T = K Q^T leaves a query's scores in one lane and its other half: the softmax needs one exchange per tile, and P^T is the next
 // product's operand as it stands (O^T = V^T P^T).  P is rounded to the inputs' type for that product (half a step, independent from key to key, so about
-// as much as the output's own rounding); its sum stays float32.
+// as much as the output's own rounding; in float16 lifted by 2^15, or one key that draws nearly all the weight and has no value would leave the others' below the
+// type's normal range); its sum stays float32.
 // Keys run from the diagonal to the first one.  The tiles that hide keys come first, in a loop of their own, and the others run without a mask.
 // Bound by LDS (32 KB a wavefront and tile for 1 024 clocks of matrix work) and the exponentials, which only the second wavefront of the SIMD hides.  One
 // sequence of 16 384 tokens, 16 heads of 128 over 4, bf16: 1.10 to 1.13 ms, 975 to 1 000 TFLOP/s (a library product of 8 192^3: 1 138); with the masks and the test for
@@ -170,7 +171,7 @@ __global__ __launch_bounds__(64 * NW, (waves_forward<T, DP, NW>)) void attention
             for (int i = 0; i < 16; ++i) s[n][i] = k0 + 32 * n + row_of(i, h) <= limit ? s[n][i] : -__builtin_inff();
         softmax(s);
 #pragma unroll
-        for (int n = 0; n < NB; ++n) add_columns<T, DP>(lds_v, 32 * n, s[n], o, lane);
+        for (int n = 0; n < NB; ++n) add_columns<T, DP>(lds_v, 32 * n, s[n], o, lane, WEIGHT<T>);
         if (nonfinite == kt + 1) {
             for (int b = 0; b < DP; b += 64) {
                 int plus, minus;
@@ -202,11 +203,11 @@ __global__ __launch_bounds__(64 * NW, (waves_forward<T, DP, NW>)) void attention
         scores(s);
         softmax(s);
 #pragma unroll
-        for (int n = 0; n < NB; ++n) add_columns<T, DP>(lds_v, 32 * n, s[n], o, lane);
+        for (int n = 0; n < NB; ++n) add_columns<T, DP>(lds_v, 32 * n, s[n], o, lane, WEIGHT<T>);
     }
     l += other_half(l);
     if (row < w.length) {
-        store_row<T>((T *)(p.o.p + (int64_t)(w.start + row) * p.o.ts + head * p.o.hs), o, l == 0.f ? 0.f : 1.f / l, d, lane);
+        store_row<T>((T *)(p.o.p + (int64_t)(w.start + row) * p.o.ts + head * p.o.hs), o, l == 0.f ? 0.f : 1.f / (l * WEIGHT<T>), d, lane);
         if (h == 0) p.lse[(int64_t)(w.start + row) * p.heads + head] = (mu + log2_(l)) * LN2;
     }
 }
@@ -398,7 +399,7 @@ __global__ __launch_bounds__(64 * NW, (waves_dkv<T, DP>)) void attention_dkv_ker
         if (t < BQ) {
             float lse = t < n ? p.lse[(at + t) * p.heads + head] : -__builtin_inff();
             delta_r = t < n ? p.delta[(at + t) * p.heads + head] : 0.f;
-            mu_r = lse == -__builtin_inff() ? __builtin_inff() : lse * LOG2E;
+            mu_r = lse == -__builtin_inff() ? __builtin_inff() : __builtin_fmaf(lse, LOG2E, -LIFT<T>);     // (P comes lifted)
         }
     };
     auto fetch_g = [&](int head, int qt) {
@@ -514,7 +515,10 @@ __global__ __launch_bounds__(64 * NW, (waves_dkv<T, DP>)) void attention_dkv_ker
     }
     if constexpr (narrow<T>) {
 #pragma unroll
-        for (int b = 0; b < DB; ++b) dk[b] *= inverse(f);
+        for (int b = 0; b < DB; ++b) {
+            dk[b] *= inverse(f) * (1.f / WEIGHT<T>);
+            dv[b] *= 1.f / WEIGHT<T>;
+        }
     }
     if (NW == 4 && p.parts > 1) {
         float *to = p.partial + (((int64_t)(w.start + key) * p.kv_heads + kvh) * p.parts + part) * 2 * DP;
@@ -572,7 +576,7 @@ __global__ __launch_bounds__(512, 2) void attention_dkv_pair_kernel(AttentionPar
         if (t < BQ) {
             float lse = t < n ? p.lse[(at + t) * p.heads + head] : -__builtin_inff();
             delta_r = t < n ? p.delta[(at + t) * p.heads + head] : 0.f;
-            mu_r = lse == -__builtin_inff() ? __builtin_inff() : lse * LOG2E;
+            mu_r = lse == -__builtin_inff() ? __builtin_inff() : __builtin_fmaf(lse, LOG2E, -LIFT<T>);     // (P comes lifted)
         }
     };
     auto put = [&]() {
@@ -691,7 +695,10 @@ __global__ __launch_bounds__(512, 2) void attention_dkv_pair_kernel(AttentionPar
     };
     if constexpr (narrow<T>) {      // (each of the two wavefronts has a lift of its own)
 #pragma unroll
-        for (int b = 0; b < DB; ++b) dk[b] *= inverse(f);
+        for (int b = 0; b < DB; ++b) {
+            dk[b] *= inverse(f) * (1.f / WEIGHT<T>);
+            dv[b] *= 1.f / WEIGHT<T>;
+        }
     }
     join(dk);
     join(dv);
@@ -839,7 +846,7 @@ __global__ __launch_bounds__(64, DP == 32 ? 2 : 1) void attention_short_grad_ker
                 for (int s = 0; s < 2; ++s) f[s] = to_frag<T>(z, s);
             } else {
 #pragma unroll
-                for (int i = 0; i < 16; ++i) *(T *)(lds_w + square::at(row_of(i, h), r / square::CE) + r % square::CE * (int)sizeof(T)) = (T)x[y][i];
+                for (int i = 0; i < 16; ++i) *(T *)(lds_w + square::at(row_of(i, h), r / square::CE) + r % square::CE * (int)sizeof(T)) = (T)(x[y][i] * (y == 0 ? WEIGHT<T> : 1.f));
                 __syncthreads();
 #pragma unroll
                 for (int s = 0; s < 2; ++s) f[s] = square::rows_permuted(lds_w, 0, 16 * s, lane);
@@ -855,7 +862,10 @@ __global__ __launch_bounds__(64, DP == 32 ? 2 : 1) void attention_short_grad_ker
     }
     if constexpr (narrow<T>) {
 #pragma unroll
-        for (int b = 0; b < DB; ++b) dk[b] *= inverse(fk);
+        for (int b = 0; b < DB; ++b) {
+            dk[b] *= inverse(fk);
+            dv[b] *= 1.f / WEIGHT<T>;
+        }
     }
     if (r < length) {
         if (r <= bad_query) {       // (a key that such a query sees: its gradients are not finite)

@@ -128,7 +128,7 @@ __global__ __launch_bounds__(64 * NW, sizeof(T) == 2 ? 2 : 1) void attention_ste
         }
 #pragma unroll
         for (int x = 0; x < 2; ++x) {
-            frag<T> pf = to_frag<T>(s[0], x);
+            frag<T> pf = to_frag<T>(s[0] * WEIGHT<T>, x);
 #pragma unroll
             for (int y = 0; y < DB; ++y) o[y] = mma(tile::cols(mine, 16 * x, 32 * y, lane), pf, o[y]);
         }
@@ -165,7 +165,7 @@ __global__ __launch_bounds__(64 * NW, sizeof(T) == 2 ? 2 : 1) void attention_ste
             a += *(const f32x4 *)(so + (y * cols + g) * DP + x) * f;
         }
         if (p.pieces == 1) {
-            const float f = L == 0.f ? 0.f : 1.f / L;
+            const float f = L == 0.f ? 0.f : 1.f / (L * WEIGHT<T>);
             if (x < d) store4((T *)(p.o.p + b * p.o.ts + (head0 + g) * p.o.hs) + x, a[0] * f, a[1] * f, a[2] * f, a[3] * f);
         } else {
             const int64_t at = ((int64_t)b * p.heads + head0 + g) * p.pieces + blockIdx.y;
@@ -212,7 +212,7 @@ __global__ __launch_bounds__(64) void attention_join_kernel(StepParams p) {
 #pragma unroll
         for (int j = 0; j < 4; ++j) a[j] += __shfl_xor(a[j], i);
     }
-    const float f = L == 0.f ? 0.f : 1.f / L;
+    const float f = L == 0.f ? 0.f : 1.f / (L * WEIGHT<T>);
     if (s == 0 && x < p.dim) store4((T *)(p.o.p + b * p.o.ts + head * p.o.hs) + x, a[0] * f, a[1] * f, a[2] * f, a[3] * f);
 }
 

@@ -98,6 +98,9 @@ template <typename T, int N> __device__ __forceinline__ void lift(f32x16 &x, flo
         x *= f;
     }
 }
+// A weight of a softmax is at most 1 (and its rounding more): always lifted by 2^15, the sum lowered by as much
+template <typename T> constexpr float LIFT = narrow<T> ? 15.f : 0.f;
+template <typename T> constexpr float WEIGHT = narrow<T> ? 32768.f : 1.f;
 template <typename T> constexpr float lift_start = narrow<T> ? 18446744073709551616.f : 1.f;
 
 // ---- LDS tiles: rows of DP elements (the head dimension padded with zeros to 32, 64, 96 or 128; 96 in the room of 128), 16-byte chunks exchanged inside each row by an XOR that
