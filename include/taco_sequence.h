@@ -22,7 +22,7 @@
 extern "C" {
 #endif
 
-#define TACO_SEQUENCE_ABI_VERSION 1
+#define TACO_SEQUENCE_ABI_VERSION 2
 
 enum { TACO_SEQ_OK = 0, TACO_SEQ_ERR_INVALID_ARG = -1, TACO_SEQ_ERR_HIP = -2, TACO_SEQ_ERR_WORKSPACE = -3 };
 enum { TACO_SEQ_F32 = 0, TACO_SEQ_F16 = 1, TACO_SEQ_BF16 = 2 };
@@ -56,7 +56,7 @@ typedef struct taco_attention_args {
     taco_seq_tensor d_o, d_q, d_k, d_v;
     float *delta;                       /* workspace [tokens][heads]: scale * rowsum(d_o o) */
     int32_t parts;                      /* 128-row tiles: a key-value head's group of query heads in that many parts (a divisor of heads / kv_heads), each a
-                                           workgroup of its own; more than 1 needs the workspace [tokens][kv_heads][parts][2][dim rounded up to a multiple of 32] */
+                                           workgroup of its own; more than 1 needs the workspace [n_tiles][128][kv_heads][parts][2][dim rounded up to a multiple of 32] */
     float *partial;
 } taco_attention_args;
 int taco_attention(const taco_attention_args *a, void *stream);

@@ -16,7 +16,7 @@ struct AttentionParams {
     const taco_seq_tile *tiles, *key_tiles;
     int32_t n_tiles, heads, kv_heads, dim, causal, parts;
     float scale;
-    float *partial;          // [tokens][kv_heads][parts][2][DP]
+    float *partial;          // [n_tiles][128][kv_heads][parts][2][DP], by the key tiles' order
 };
 
 // Workgroups go to the 8 XCDs in turn, each with an L2 of its own: with a multiple of 8 heads, neighbouring heads (one group's, which read the same keys and
@@ -521,7 +521,7 @@ __global__ __launch_bounds__(64 * NW, (waves_dkv<T, DP>)) void attention_dkv_ker
         }
     }
     if (NW == 4 && p.parts > 1) {
-        float *to = p.partial + (((int64_t)(w.start + key) * p.kv_heads + kvh) * p.parts + part) * 2 * DP;
+        float *to = p.partial + ((((int64_t)ti * 128 + key - w.first) * p.kv_heads + kvh) * p.parts + part) * 2 * DP;
         if (key < w.length) {
             store_row<float>(to, dk, 1.f, DP, lane);
             store_row<float>(to + DP, dv, 1.f, DP, lane);
@@ -704,7 +704,7 @@ __global__ __launch_bounds__(512, 2) void attention_dkv_pair_kernel(AttentionPar
     join(dv);
     if (half || key >= w.length) return;
     if (p.parts > 1) {
-        float *to = p.partial + (((int64_t)(w.start + key) * p.kv_heads + kvh) * p.parts + part) * 2 * DP;
+        float *to = p.partial + ((((int64_t)ti * 128 + key - w.first) * p.kv_heads + kvh) * p.parts + part) * 2 * DP;
         store_row<float>(to, dk, 1.f, DP, lane);
         store_row<float>(to + DP, dv, 1.f, DP, lane);
     } else {
@@ -721,7 +721,7 @@ template <typename T, int DP> __global__ __launch_bounds__(256) void attention_s
     for (int e = threadIdx.x; e < rows * (DP / 4); e += 256) {
         const int64_t token = w.start + w.first + e / (DP / 4);
         const int x = e % (DP / 4) * 4;
-        const float *from = p.partial + (token * p.kv_heads + kvh) * p.parts * 2 * DP + x;
+        const float *from = p.partial + (((int64_t)ti * 128 + e / (DP / 4)) * p.kv_heads + kvh) * p.parts * 2 * DP + x;
         f32x4 dk{0, 0, 0, 0}, dv{0, 0, 0, 0};
         for (int i = 0; i < p.parts; ++i) {
             dk += *(const f32x4 *)(from + i * 2 * DP);

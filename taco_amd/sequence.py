@@ -27,7 +27,7 @@ from torch.autograd import forward_ad
 
 from . import _lib
 
-ABI_VERSION = 1
+ABI_VERSION = 2
 EXPORTS = ["taco_sequence_abi_version", "taco_sequence_source_hash", "taco_sequence_last_error", "taco_attention", "taco_attention_backward",
            "taco_attention_step_workspace_bytes", "taco_attention_step", "taco_linear_attention_workspace_bytes", "taco_linear_attention",
            "taco_linear_attention_backward", "taco_linear_attention_step"]
@@ -237,13 +237,17 @@ class Packed:
                     t.record_stream(torch.cuda.current_stream(self.device))
         return got[0]
 
+    def _wide(self, heads):
+        """whether there are tiles of 128 rows: if those alone fill the CUs"""
+        return self._wide_tiles * heads >= 256
+
     def _tiles(self, heads):
         """[(tile rows, tiles, key tiles, count, how many of them at the end are whole sequences)].  A tile of 128 rows shares its loads between four wavefronts;
         sequences of at most 64 tokens would leave half of it idle, and where all tiles together do not fill the CUs, smaller ones spread the work.  Sequences
         of at most 32 tokens are a tile each.  A few short sequences beside many long ones take a 128-row tile each all the same: launches of their own would
         run on some CUs after the others (100 sequences of 65 to 200 tokens, 8 heads of 128 over 2, and 30 of up to 64, forward and backward: bf16 283 -> 229 us,
         float32 1.03 -> 0.79 ms; with 120 short ones 323 -> 313 us; with 250 they would cost 351 -> 388)."""
-        wide = self._wide_tiles * heads >= 256
+        wide = self._wide(heads)
         few = wide and self._short * heads <= _FEW_SHORT
         key = "wide tiles only" if few else "wide tiles" if wide else "tiles"
 
@@ -265,7 +269,10 @@ class Packed:
 
     def _parts(self, heads, group, causal):
         """Into how many parts the backward's second launch shares out a group's query heads: few enough that their partial sums' way through memory stays small, but
-        so many that the longest sequence's first tile of keys, which sees all its queries, takes no longer than a CU's share of everything."""
+        so many that the longest sequence's first tile of keys, which sees all its queries, takes no longer than a CU's share of everything.  (Only tiles of 128
+        rows are: with others alone there is one part, and no memory for sums.)"""
+        if not self._wide(heads):
+            return 1
         share = self._pairs * (0.5 if causal else 1.0) * heads / 128 / 256
         for parts in range(1, group + 1):
             if group % parts == 0 and self._longest * (group // parts) <= share:
@@ -375,9 +382,10 @@ class _Attention(torch.autograd.Function):
             delta = torch.empty(q.shape[:2], dtype=torch.float32, device=q.device)
             a.d_o, a.d_q, a.d_k, a.d_v, a.delta = _tensor(d_o), _tensor(dq), _tensor(dk), _tensor(dv), delta.data_ptr()
             H, Hk, d = q.shape[1], k.shape[1], q.shape[2]
-            a.parts = 1 if H == Hk else seqs._parts(H, H // Hk, causal)
+            a.parts = seqs._parts(H, H // Hk, causal)
             if a.parts > 1:
-                partial = torch.empty((seqs.total, Hk, a.parts, 2, -(-d // 32) * 32), dtype=torch.float32, device=q.device)
+                wide = seqs._tiles(H)[0][3]
+                partial = torch.empty((wide * 128, Hk, a.parts, 2, -(-d // 32) * 32), dtype=torch.float32, device=q.device)
                 a.partial = partial.data_ptr()
             _launch_tiles(a, seqs, q.device, True)
         return dq, dk, dv, None, None, None

@@ -315,3 +315,12 @@ def test_tangents_and_scales_that_want_a_gradient_are_refused():
             f(torch.tensor(0.5, requires_grad=True))
     with torch.no_grad():
         assert s._scale(torch.tensor(0.5, requires_grad=True), 32, True) == 0.5
+
+
+def test_sums_of_parts_only_where_tiles_of_128_rows_are():
+    """a group's heads are shared out in the launch of the wide tiles alone; elsewhere no memory is asked for their sums"""
+    for lens, heads, group in (([32] * 4096, 32, 8), ([64] * 4096, 16, 4), ([2000], 8, 8), ([5, 0, 31], 4, 2), ([], 4, 4), ([700, 129], 64, 32), ([700, 129], 64, 1)):
+        seqs = sequence.Packed(lens, "cuda:0")
+        wide = -(-np.array([n for n in lens if n > 64] + [0]) // 128).sum() * heads >= 256
+        assert seqs._wide(heads) == wide and (wide or seqs._parts(heads, group, True) == seqs._parts(heads, group, False) == 1)
+    assert sequence.Packed([700, 129], "cuda:0")._parts(64, 32, True) > 1
