@@ -49,7 +49,8 @@ typedef struct taco_attention_args {
     const taco_seq_tile *tiles;
     const taco_seq_tile *key_tiles;     /* backward: the same tiles in the order their keys want (most queries first), or NULL */
     int32_t n_tiles, tile_rows;
-    int32_t whole;                      /* not 0: every tile is a whole sequence, of at most tile_rows = 32 tokens (longer ones are cut off there) */
+    int32_t whole;                      /* backward: not 0: every tile is a whole sequence, of at most tile_rows = 32 tokens (longer ones are cut off there); not
+                                           for float32 with dim > 96, which is refused */
     int32_t heads, kv_heads, dim, dtype, causal;
     float scale;                        /* > 0 */
     /* backward only: */
@@ -61,7 +62,7 @@ typedef struct taco_attention_args {
 } taco_attention_args;
 int taco_attention(const taco_attention_args *a, void *stream);
 /* Gradients by the formulas (P from lse; dS = P (dP - rowsum(d_o o))): two launches, the second reads `delta`, which the first writes; one launch where
- * the tiles are whole sequences (o and delta are not read then). */
+ * the tiles are whole sequences (o and delta have to be given then too, but are neither read nor written). */
 int taco_attention_backward(const taco_attention_args *a, void *stream);
 
 /* ---- Attention of one new token per row over a paged cache, which the token joins.

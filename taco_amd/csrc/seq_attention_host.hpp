@@ -10,6 +10,7 @@ inline int attention_params(const taco_attention_args *a, bool backward, Attenti
     SEQ_NEED(a->scale > 0.f && a->scale < __builtin_inff(), "scale %g: positive and finite", (double)a->scale);
     SEQ_NEED(a->tile_rows == 32 || a->tile_rows == 128, "tile_rows %d: 32 or 128", a->tile_rows);
     SEQ_NEED(!a->whole || a->tile_rows == 32, "whole sequences: tile_rows 32, not %d", a->tile_rows);
+    SEQ_NEED(!backward || !a->whole || a->dtype != TACO_SEQ_F32 || a->dim <= 96, "whole sequences of float32 rows of %d: at most 96", a->dim);
     SEQ_NEED(a->n_tiles >= 0 && (int64_t)a->n_tiles * a->heads < (int64_t)1 << 31, "%d tiles of %d heads: fewer than 2^31 in all", a->n_tiles, a->heads);
     p = AttentionParams{};
     p.n_tiles = a->n_tiles;

@@ -328,6 +328,8 @@ def _launch_tiles(a, seqs, device, backward):
         if not backward:
             _call(lib.taco_attention, a, device)
             continue
+        if a.dtype == 0 and a.dim > 96:     # (float32 rows this wide: no form for whole sequences)
+            whole = 0
         a.n_tiles = count - whole           # (whole sequences have a launch of their own)
         if a.n_tiles:
             _call(lib.taco_attention_backward, a, device)

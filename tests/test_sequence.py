@@ -324,3 +324,23 @@ def test_sums_of_parts_only_where_tiles_of_128_rows_are():
         wide = -(-np.array([n for n in lens if n > 64] + [0]) // 128).sum() * heads >= 256
         assert seqs._wide(heads) == wide and (wide or seqs._parts(heads, group, True) == seqs._parts(heads, group, False) == 1)
     assert sequence.Packed([700, 129], "cuda:0")._parts(64, 32, True) > 1
+
+
+def test_whole_sequences_where_no_such_form_is(lib):
+    """float32 rows above 96 have no one-launch gradients: the flag is refused, and the host layer does not set it"""
+    for dim, code in ((96, 0), (104, -1), (128, -1)):
+        wide = {f: tensor(ts=2 * dim, hs=dim) for f in ("q", "k", "v", "o", "d_o", "d_q", "d_k", "d_v")}
+        a = attention_args(whole=1, tile_rows=32, dim=dim, n_tiles=0 if code == 0 else 1, **wide)
+        assert lib.taco_attention_backward(C.byref(a), None) == code
+        assert code == 0 or b"whole" in lib.taco_sequence_last_error()
+
+
+@pytest.mark.parametrize("dtype,dim,flags", [(0, 96, [0, 1]), (0, 128, [0]), (1, 128, [0, 1]), (2, 128, [0, 1])])
+def test_launches_of_the_gradients(monkeypatch, dtype, dim, flags):
+    seqs, seen = lists(monkeypatch, [40, 5, 33, 32]), []
+    monkeypatch.setattr(sequence.Packed, "_tiles", lambda self, heads, f=sequence.Packed._tiles: [(r, torch.from_numpy(t), torch.from_numpy(k), n, w) for r, t, k, n, w in f(self, heads)])
+    monkeypatch.setattr(sequence, "_call", lambda f, a, device: seen.append((a.whole, a.n_tiles, a.tiles)))
+    a = attention_args(dtype=dtype, dim=dim)
+    sequence._launch_tiles(a, seqs, torch.device("cuda:0"), True)
+    assert [x[0] for x in seen] == flags and sum(x[1] for x in seen) == 6
+    assert len(seen) == 1 or seen[1][2] - seen[0][2] == 16 * seen[0][1]
