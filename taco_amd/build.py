@@ -38,7 +38,7 @@ FLAGS = ["--offload-arch=gfx950", "-O3", "-std=c++17", "-fPIC", "-shared", "-ffp
 # multiply-adds are the compiler's choice here (no bit contract with a CPU restatement); no packed float32 arithmetic.
 LIB_SEQ = os.path.join(HERE, "libtaco_sequence.so")
 SEQ_SOURCES = ["seq_common.hip", "seq_attention.hip", "seq_attention_grad.hip", "seq_attention_step.hip", "seq_linear.hip"]
-SEQ_DEPS = SEQ_SOURCES + ["seq_core.hpp", "seq_host.hpp", "seq_attention.hpp", "seq_attention_host.hpp", "seq_attention_step.hpp", "seq_pages.hpp", "seq_linear.hpp",
+SEQ_DEPS = SEQ_SOURCES + ["seq_core.hpp", "seq_host.hpp", "seq_attention.hpp", "seq_attention_host.hpp", "seq_attention_step.hpp", "seq_pages.hpp", "seq_launches.hpp", "seq_linear.hpp",
                           os.path.join("..", "..", "include", "taco_sequence.h")]
 SEQ_FLAGS = ["--offload-arch=gfx950", "-O3", "-std=c++17", "-fPIC", "-fvisibility=hidden", "-fno-exceptions", "-fno-strict-aliasing", "-fno-slp-vectorize",
              "-Xclang", "-target-feature", "-Xclang", "-packed-fp32-ops", "-Wall", "-Wno-unused-function"]

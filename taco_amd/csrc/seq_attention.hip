@@ -9,9 +9,11 @@ SEQ_API int taco_attention(const taco_attention_args *a, void *stream) {
     return dispatch(a->dtype, a->dim, [&](auto type, auto dp) {
         typedef decltype(type) T;
         constexpr int DP = decltype(dp)::value;
-        const dim3 grid((unsigned)(p.n_tiles * p.heads));
-        if (a->tile_rows == 32) attention_kernel<T, DP, 1><<<grid, 64, 0, (hipStream_t)stream>>>(p);
-        else attention_kernel<T, DP, 4><<<grid, 256, 0, (hipStream_t)stream>>>(p);
+        in_launches((int64_t)p.n_tiles * p.heads, 2 * a->tile_rows, [&](int32_t first, uint32_t grid) {
+            p.first_block = first;
+            if (a->tile_rows == 32) attention_kernel<T, DP, 1><<<grid, 64, 0, (hipStream_t)stream>>>(p);
+            else attention_kernel<T, DP, 4><<<grid, 256, 0, (hipStream_t)stream>>>(p);
+        });
         return launched("taco_attention");
     });
 }

@@ -14,7 +14,7 @@ struct AttentionParams {
     View q, k, v, o, d_o, d_q, d_k, d_v;
     float *lse, *delta;
     const taco_seq_tile *tiles, *key_tiles;
-    int32_t n_tiles, heads, kv_heads, dim, causal, parts;
+    int32_t n_tiles, heads, kv_heads, dim, causal, parts, first_block;      // first_block: of this launch
     float scale;
     float *partial;          // [n_tiles][128][kv_heads][parts][2][DP], by the key tiles' order
 };
@@ -81,7 +81,7 @@ __global__ __launch_bounds__(64 * NW, (waves_forward<T, DP, NW>)) void attention
     __shared__ __attribute__((aligned(16))) char lds_k[BN * tile::ROW], lds_v[BN * tile::ROW];
     __shared__ int nonfinite;
     int ti, head;
-    locate(blockIdx.x, p.heads, ti, head);
+    locate(p.first_block + blockIdx.x, p.heads, ti, head);
     const taco_seq_tile w = p.tiles[ti];
     const int kvh = head / (p.heads / p.kv_heads), t = threadIdx.x, lane = t & 63, wave = __builtin_amdgcn_readfirstlane(t >> 6), h = lane >> 5, d = p.dim;
     const int first = w.first + 32 * wave, row = first + (lane & 31);
@@ -227,7 +227,7 @@ __global__ __launch_bounds__(64 * NW, (waves_dq<T, DP, NW>)) void attention_dq_k
     __shared__ __attribute__((aligned(16))) char lds_k[BN * tile::ROW], lds_v[BN * tile::ROW];
     __shared__ int nonfinite;       // the first key of the tile with something not finite in it
     int ti, head;
-    locate(blockIdx.x, p.heads, ti, head);
+    locate(p.first_block + blockIdx.x, p.heads, ti, head);
     const taco_seq_tile w = p.tiles[ti];
     const int kvh = head / (p.heads / p.kv_heads), t = threadIdx.x, lane = t & 63, wave = __builtin_amdgcn_readfirstlane(t >> 6), h = lane >> 5, d = p.dim;
     const int first = w.first + 32 * wave, row = first + (lane & 31);
@@ -367,7 +367,7 @@ __global__ __launch_bounds__(64 * NW, (waves_dkv<T, DP>)) void attention_dkv_ker
     __shared__ __attribute__((aligned(16))) float lds_mu[BQ], lds_delta[BQ];
     __shared__ int nonfinite;       // the last query of the tile with something not finite in its row or its gradient's
     int ti, kvh;
-    locate(blockIdx.x, p.kv_heads * p.parts, ti, kvh);
+    locate(p.first_block + blockIdx.x, p.kv_heads * p.parts, ti, kvh);
     const int part = kvh % p.parts;
     kvh /= p.parts;
     const taco_seq_tile w = p.key_tiles[ti];
@@ -547,7 +547,7 @@ __global__ __launch_bounds__(512, 2) void attention_dkv_pair_kernel(AttentionPar
     char *const lds_k = lds, *const lds_v = lds + KT, *const lds_q = lds + 2 * KT, *const lds_g = lds + 2 * KT + QT;
     static_assert(4 * DB * 16 * 64 * sizeof(float) <= sizeof(lds), "the sums of four wavefronts");
     int ti, kvh;
-    locate(blockIdx.x, p.kv_heads * p.parts, ti, kvh);
+    locate(p.first_block + blockIdx.x, p.kv_heads * p.parts, ti, kvh);
     const int part = kvh % p.parts;
     kvh /= p.parts;
     const taco_seq_tile w = p.key_tiles[ti];
@@ -715,7 +715,7 @@ __global__ __launch_bounds__(512, 2) void attention_dkv_pair_kernel(AttentionPar
 
 template <typename T, int DP> __global__ __launch_bounds__(256) void attention_sum_kernel(AttentionParams p) {
     int ti, kvh;
-    locate(blockIdx.x, p.kv_heads, ti, kvh);
+    locate(p.first_block + blockIdx.x, p.kv_heads, ti, kvh);
     const taco_seq_tile w = p.key_tiles[ti];
     const int rows = min(128, w.length - w.first);
     for (int e = threadIdx.x; e < rows * (DP / 4); e += 256) {
@@ -748,7 +748,7 @@ __global__ __launch_bounds__(64, DP == 32 ? 2 : 1) void attention_short_grad_ker
     constexpr int NS = DP / 16, DB = DP / 32;
     __shared__ __attribute__((aligned(16))) char lds_k[32 * tile::ROW], lds_q[32 * tile::ROW], lds_g[32 * tile::ROW], lds_w[32 * (narrow<T> ? square32::ROW : square::ROW)];
     int ti, kvh;
-    locate(blockIdx.x, p.kv_heads, ti, kvh);
+    locate(p.first_block + blockIdx.x, p.kv_heads, ti, kvh);
     const taco_seq_tile w = p.key_tiles[ti];
     const int lane = threadIdx.x, h = lane >> 5, r = lane & 31, d = p.dim, G = p.heads / p.kv_heads, length = min(w.length, 32);
     const uint32_t rb = d * sizeof(T);

@@ -88,11 +88,18 @@ SEQ_API int taco_attention_step(const taco_attention_step_args *a, void *stream)
         p.part_o = (float *)a->workspace;
         p.part_ml = p.part_o + (int64_t)p.rows * p.heads * p.pieces * DP;
         const int nw = few ? 1 : 4, tiles = nw * 32 * Tile<T, DP>::ROW, join = nw * cols * (DP + 2) * (int)sizeof(float);
-        const dim3 grid((unsigned)((int64_t)p.rows * p.kv_heads * p.blocks), (unsigned)p.pieces);
         const size_t lds = tiles > join ? tiles : join;
-        if (few) attention_step_kernel<T, DP, 1><<<grid, 64, lds, (hipStream_t)stream>>>(p);
-        else attention_step_kernel<T, DP, 4><<<grid, 256, lds, (hipStream_t)stream>>>(p);
-        if (p.pieces > 1) attention_join_kernel<T, DP><<<dim3((unsigned)(p.rows * p.heads)), 64, 0, (hipStream_t)stream>>>(p);
+        in_launches((int64_t)p.rows * p.kv_heads * p.blocks, 64 * nw, [&](int32_t first, uint32_t n) {
+            const dim3 grid(n, (unsigned)p.pieces);
+            p.first_block = first;
+            if (few) attention_step_kernel<T, DP, 1><<<grid, 64, lds, (hipStream_t)stream>>>(p);
+            else attention_step_kernel<T, DP, 4><<<grid, 256, lds, (hipStream_t)stream>>>(p);
+        });
+        if (p.pieces > 1)
+            in_launches((int64_t)p.rows * p.heads, 64, [&](int32_t first, uint32_t n) {
+                p.first_block = first;
+                attention_join_kernel<T, DP><<<n, 64, 0, (hipStream_t)stream>>>(p);
+            });
         return launched("taco_attention_step");
     });
 }

@@ -12,7 +12,7 @@ struct StepParams {
     const int32_t *table, *lengths;
     int64_t table_stride;
     int32_t rows, table_width, num_pages, page_size, heads, kv_heads, dim, blocks;      // blocks: of 32 query heads in a group
-    int32_t piece, pieces;
+    int32_t piece, pieces, first_block;     // first_block: of this launch
     float scale;
     float *part_o, *part_ml;            // [rows][heads][pieces][DP], [rows][heads][pieces][2]
 };
@@ -28,7 +28,7 @@ __global__ __launch_bounds__(64 * NW, sizeof(T) == 2 ? 2 : 1) void attention_ste
     constexpr int NS = DP / 16, DB = DP / 32, N = 32 * tile::NC / 64;
     extern __shared__ __attribute__((aligned(16))) char lds[];
     const int t = threadIdx.x, lane = t & 63, wave = t >> 6, h = lane >> 5, d = p.dim;
-    const int blk = blockIdx.x % p.blocks, kvh = blockIdx.x / p.blocks % p.kv_heads, b = blockIdx.x / p.blocks / p.kv_heads;
+    const int block = p.first_block + blockIdx.x, blk = block % p.blocks, kvh = block / p.blocks % p.kv_heads, b = block / p.blocks / p.kv_heads;
     const int G = p.heads / p.kv_heads, g0 = 32 * blk, cols = min(32, G - g0), head0 = kvh * G + g0;
     const bool joins = p.k_new.p != nullptr;
     const int len = p.lengths[b], keys = keys_of(len, p.table_width, p.page_size, joins);
@@ -192,9 +192,9 @@ __global__ __launch_bounds__(64 * NW, sizeof(T) == 2 ? 2 : 1) void attention_ste
 template <typename T, int DP>
 __global__ __launch_bounds__(64) void attention_join_kernel(StepParams p) {
     constexpr int W = DP == 96 ? 32 : DP / 4, S = 64 / W;
-    const int b = blockIdx.x / p.heads, head = blockIdx.x % p.heads, lane = threadIdx.x, x = lane % W * 4, s = lane / W;
+    const int block = p.first_block + blockIdx.x, b = block / p.heads, head = block % p.heads, lane = threadIdx.x, x = lane % W * 4, s = lane / W;
     const int n = pieces_of(keys_of(p.lengths[b], p.table_width, p.page_size, p.k_new.p != nullptr), p.piece);
-    const int64_t at = (int64_t)blockIdx.x * p.pieces;
+    const int64_t at = (int64_t)block * p.pieces;
     float M = -__builtin_inff();
     for (int i = lane; i < n; i += 64) M = fmaxf(M, p.part_ml[(at + i) * 2]);
 #pragma unroll

@@ -1,6 +1,7 @@
 // Host side shared by the entry points of taco_sequence.h: argument checks, errors, type dispatch.
 #pragma once
 #include "seq_attention.hpp"
+#include "seq_launches.hpp"
 
 namespace seq {
 

@@ -34,12 +34,17 @@ static int run(const taco_linear_attention_args *a, LinearParams &p, int modes, 
     return dispatch(a->dtype, a->dim, [&](auto type, auto dp) {
         typedef decltype(type) T;
         constexpr int DP = decltype(dp)::value;
-        const dim3 grid((unsigned)p.n_segments, (unsigned)p.heads, (unsigned)modes);
+        auto segments = [&](int threads, auto kernel) {
+            in_launches(p.n_segments, threads, [&](int32_t first, uint32_t n) {
+                p.first_block = first;
+                kernel<<<dim3(n, (unsigned)p.heads, (unsigned)modes), threads, 0, (hipStream_t)stream>>>(p);
+            });
+        };
         if (p.carry) {
-            linear_kernel<T, DP, true><<<grid, 2 * DP * (chunk_of<T> / 32), 0, (hipStream_t)stream>>>(p);
+            segments(2 * DP * (chunk_of<T> / 32), linear_kernel<T, DP, true>);
             linear_scan_kernel<DP><<<dim3(DP * DP / 256, (unsigned)(p.n_sequences * p.heads), (unsigned)modes), 256, 0, (hipStream_t)stream>>>(p);
         }
-        linear_kernel<T, DP, false><<<grid, 4 * DP, 0, (hipStream_t)stream>>>(p);
+        segments(4 * DP, linear_kernel<T, DP, false>);
         return launched("taco_linear_attention");
     });
 }
@@ -112,9 +117,11 @@ SEQ_API int taco_linear_attention_step(const taco_linear_attention_step_args *a,
     p.heads = a->heads;
     p.dim = a->dim;
     p.scale = a->scale;
-    const unsigned grid = (unsigned)(a->rows * a->heads);
-    if (a->dtype == TACO_SEQ_F32) linear_step_kernel<float><<<grid, 256, 0, (hipStream_t)stream>>>(p);
-    else if (a->dtype == TACO_SEQ_F16) linear_step_kernel<f16><<<grid, 256, 0, (hipStream_t)stream>>>(p);
-    else linear_step_kernel<bf16><<<grid, 256, 0, (hipStream_t)stream>>>(p);
+    in_launches((int64_t)a->rows * a->heads, 256, [&](int32_t first, uint32_t grid) {
+        p.first_block = first;
+        if (a->dtype == TACO_SEQ_F32) linear_step_kernel<float><<<grid, 256, 0, (hipStream_t)stream>>>(p);
+        else if (a->dtype == TACO_SEQ_F16) linear_step_kernel<f16><<<grid, 256, 0, (hipStream_t)stream>>>(p);
+        else linear_step_kernel<bf16><<<grid, 256, 0, (hipStream_t)stream>>>(p);
+    });
     return launched("taco_linear_attention_step");
 }

@@ -24,7 +24,7 @@ struct LinearParams {
     const float *log_decay;
     const taco_seq_segment *segments;
     const int32_t *first_segment;
-    int32_t n_segments, n_sequences, heads, dim;
+    int32_t n_segments, n_sequences, heads, dim, first_block;      // first_block: of this launch, a segment
     float *carry;           // [modes][n_segments][heads][DP * DP], or NULL: one segment per sequence
 };
 
@@ -112,11 +112,12 @@ __global__ __launch_bounds__(STATES ? 2 * DP * (chunk_of<T> / 32) : 4 * DP, 2) v
     const LinearMode m = p.mode[blockIdx.z];
     const int head = blockIdx.y, t = threadIdx.x, lane = t & 63, wave = __builtin_amdgcn_readfirstlane(t >> 6), slice = wave % DB, h = lane >> 5, d = p.dim;
     const bool keeper = STATES || wave >= DB;       // of the state; else: makes the outputs
-    const taco_seq_segment g = p.segments[blockIdx.x];
+    const int segment = p.first_block + blockIdx.x;
+    const taco_seq_segment g = p.segments[segment];
     if (STATES && g.first + g.count == g.length) return;        // (nothing starts from the last segment's state)
     const uint32_t rb = d * sizeof(T);
     const float ld = decay2(p.log_decay, head);
-    float *carry = p.carry ? p.carry + (((int64_t)blockIdx.z * p.n_segments + blockIdx.x) * p.heads + head) * DP * DP : nullptr;
+    float *carry = p.carry ? p.carry + (((int64_t)blockIdx.z * p.n_segments + segment) * p.heads + head) * DP * DP : nullptr;
     const int col = 32 * slice + (lane & 31);       // this lane's value dimension
 
     Staged<T, DP, C, NT> sk, sv, sq;
@@ -371,7 +372,7 @@ struct LinearStepParams {
     const float *log_decay;
     float *state;
     const uint8_t *reset;
-    int32_t reset_bytes, rows, heads, dim;
+    int32_t reset_bytes, rows, heads, dim, first_block;
     float scale;
 };
 
@@ -380,7 +381,7 @@ struct LinearStepParams {
 template <typename T> __global__ __launch_bounds__(256) void linear_step_kernel(LinearStepParams p) {
     __shared__ float lq[128], lk[128];
     __shared__ __attribute__((aligned(16))) float lv[128], part[1024];
-    const int row = blockIdx.x / p.heads, head = blockIdx.x % p.heads, t = threadIdx.x, d = p.dim;
+    const int block = p.first_block + blockIdx.x, row = block / p.heads, head = block % p.heads, t = threadIdx.x, d = p.dim;
     if (t < d) {
         lq[t] = (float)((const T *)(p.q.p + row * p.q.ts + head * p.q.hs))[t];
         lk[t] = (float)((const T *)(p.k.p + row * p.k.ts + head * p.k.hs))[t];
@@ -391,7 +392,7 @@ template <typename T> __global__ __launch_bounds__(256) void linear_step_kernel(
         for (int i = 0; i < p.reset_bytes; ++i) fresh |= p.reset[(int64_t)row * p.reset_bytes + i] != 0;
     const float g = exp2_(decay2(p.log_decay, head));
     __syncthreads();
-    float *s = p.state + (int64_t)blockIdx.x * d * d;
+    float *s = p.state + (int64_t)block * d * d;
     const int w = d / 4, lanes = 256 / w * w, step = lanes / w, c = t % w * 4;      // w lanes across, `step` key rows at a time
     f32x4 a{0, 0, 0, 0};
     if (t < lanes) {

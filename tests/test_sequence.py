@@ -344,3 +344,31 @@ def test_launches_of_the_gradients(monkeypatch, dtype, dim, flags):
     sequence._launch_tiles(a, seqs, torch.device("cuda:0"), True)
     assert [x[0] for x in seen] == flags and sum(x[1] for x in seen) == 6
     assert len(seen) == 1 or seen[1][2] - seen[0][2] == 16 * seen[0][1]
+
+
+def test_launches_of_fewer_than_2_to_32_threads(tmp_path):
+    """seq_launches.hpp: every workgroup once, in order, and no launch whose threads pass 32 bits"""
+    src = tmp_path / "t.cpp"
+    src.write_text(r'''
+#include <cassert>
+#include <cstdio>
+#include <initializer_list>
+#include "seq_launches.hpp"
+int main() {
+    for (int threads : {64, 128, 192, 256, 384, 512})
+        for (int64_t blocks : {(int64_t)0, (int64_t)1, (int64_t)8388607, (int64_t)8388608, (int64_t)16777215, (int64_t)16777216, (int64_t)16777221, (int64_t)67108864, (int64_t)2147483647}) {
+            int64_t done = 0;
+            int calls = 0;
+            seq::in_launches(blocks, threads, [&](int32_t first, uint32_t n) {
+                assert(first == done && n > 0 && (int64_t)n * threads < (int64_t)1 << 32);
+                done += n;
+                ++calls;
+            });
+            assert(done == blocks && (calls <= 1 || blocks * threads >= (int64_t)1 << 32));
+        }
+    puts("ok");
+}
+''')
+    exe = str(tmp_path / "t")
+    subprocess.check_call(["g++", "-std=c++17", "-O1", "-g", "-fsanitize=address,undefined", "-I", os.path.join(ROOT, "taco_amd", "csrc"), "-o", exe, str(src)])
+    assert subprocess.check_output([exe]).strip() == b"ok"
