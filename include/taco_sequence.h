@@ -10,7 +10,8 @@
  * a negative status; taco_sequence_last_error() returns a thread-local message.  Everything may be captured into a HIP graph.  No sum depends on an
  * order that is not fixed: the same call gives the same bits.
  *
- * Tensors: `ptr` 16-byte aligned, the head dimension contiguous, token and head strides in ELEMENTS, multiples of 16 bytes.  All of one dtype
+ * Tensors: `ptr` 16-byte aligned, the head dimension contiguous, token and head strides in ELEMENTS, multiples of 16 bytes, token strides (and the head
+ * stride of taco_attention_step's q) at most 2^21.  All of one dtype
  * unless said otherwise.  dim: a multiple of 8, 8 .. 128.  Sums, softmax statistics and states are float32.
  */
 #ifndef TACO_SEQUENCE_H

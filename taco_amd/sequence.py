@@ -475,6 +475,8 @@ def attention_step(q, k, v, k_pages, v_pages, page_table, lengths, scale=None, o
     if not B:
         return out
     q = _usable(q)
+    if H > 1 and q.stride(1) > 1 << 21:         # (a descriptor reaches over the heads of a row)
+        q = q.contiguous()
     if k is None:
         new_k = new_v = Tensor()
     else:

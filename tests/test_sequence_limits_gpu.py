@@ -76,3 +76,13 @@ def test_attention_step_of_many_rows():
     table = torch.arange(B, device="cuda", dtype=torch.int32)[:, None] % 3
     o = S().attention_step(q, None, None, kp, vp, table, torch.ones(B, dtype=torch.int32, device="cuda"))
     assert torch.equal(o, vp[table[:, 0].long(), 0])
+
+
+def test_attention_step_heads_before_rows():
+    """a query whose heads lie farther apart than a descriptor reaches"""
+    B, H, d = 33000, 2, 64
+    q = torch.randn(H, B, d, generator=torch.Generator("cuda").manual_seed(1), device="cuda", dtype=torch.float16).transpose(0, 1)
+    assert q.stride(1) > 1 << 21
+    kp, vp = (torch.randn(1, 8, 1, d, generator=torch.Generator("cuda").manual_seed(i), device="cuda", dtype=torch.float16) for i in (2, 3))
+    args = kp, vp, torch.zeros(B, 1, dtype=torch.int32, device="cuda"), torch.arange(B, device="cuda", dtype=torch.int32) % 9
+    assert torch.equal(S().attention_step(q, None, None, *args), S().attention_step(q.contiguous(), None, None, *args))
