@@ -212,8 +212,9 @@ class Packed:
             raise _lib.TacoError("the sequence kernels run on an MI355X; device must be a cuda:N (HIP) device")
         if self.device.index is None:
             self.device = torch.device("cuda", torch.cuda.current_device())
-        self.lengths, self.starts, self.total = n, np.cumsum(n) - n, int(n.sum())
-        if self.total >= 2 ** 31 - 4096:
+        limit = 2 ** 31 - 4096              # (a length of its own first: many such wrap around in their sum)
+        self.lengths, self.starts, self.total = n, np.cumsum(n) - n, int(n.sum()) if (n < limit).all() else int(n.max())
+        if self.total >= limit:
             raise ValueError(f"{self.total} tokens: fewer than 2^31 - 4096 are supported")
         self._lists = {}
         self._wide_tiles = int((-(-n[n > 64] // 128)).sum())

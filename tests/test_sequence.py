@@ -372,3 +372,9 @@ int main() {
     exe = str(tmp_path / "t")
     subprocess.check_call(["g++", "-std=c++17", "-O1", "-g", "-fsanitize=address,undefined", "-I", os.path.join(ROOT, "taco_amd", "csrc"), "-o", exe, str(src)])
     assert subprocess.check_output([exe]).strip() == b"ok"
+
+
+@pytest.mark.parametrize("lens", [[2 ** 62] * 4, [2 ** 62] * 4 + [5], [2 ** 63 - 1, 1], [2 ** 31 - 4096], [2 ** 30] * 2, np.array([2 ** 63], np.uint64)])
+def test_lengths_whose_sum_wraps_are_refused(lens):
+    with pytest.raises(ValueError):
+        sequence.Packed(lens, "cuda:0")
