@@ -160,6 +160,8 @@ def _tensor(t):
 def _check_out(out, q):
     if out.shape != q.shape or out.dtype != q.dtype or out.device != q.device or _usable(out) is not out:
         raise ValueError("out: q's shape, dtype and device, rows of whole 16-byte chunks")
+    if out.requires_grad and torch.is_grad_enabled():       # (its graph would go on as if nothing had been written)
+        raise _lib.TacoError("out requires a gradient: what is written into it has none")
 
 
 def _scale(scale, dim, positive):

@@ -378,3 +378,13 @@ int main() {
 def test_lengths_whose_sum_wraps_are_refused(lens):
     with pytest.raises(ValueError):
         sequence.Packed(lens, "cuda:0")
+
+
+def test_an_output_that_requires_a_gradient_is_refused():
+    """the graph that made it would go on as if nothing had been written there"""
+    s, x, out = sequence, Fake((4, 2, 32)), Fake((4, 2, 32), grad=True)
+    pages, table, lens = Fake((6, 16, 2, 32)), Fake((4, 3), torch.int32), Fake((4,), torch.int32)
+    for f in (lambda: s.attention(x, x, x, s.Packed([4], "cuda:0"), out=out), lambda: s.attention_step(x, x, x, pages, pages, table, lens, out=out),
+              lambda: s.linear_attention_step(x, x, x, Fake((2,)), Fake((4, 2, 32, 32)), out=out)):
+        with pytest.raises(_lib.TacoError, match="out requires a gradient"):
+            f()
