@@ -105,7 +105,7 @@ typedef struct taco_linear_attention_args {
     const int32_t *first_segment;       /* [n_sequences + 1] */
     int32_t n_segments, n_sequences;
     int32_t heads, dim, dtype;
-    float scale;                        /* finite, not 0 */
+    float scale;                        /* finite, at least 2^-126 in size (the gradients' states are divided by it) */
     void *workspace;
     size_t workspace_bytes;
     /* backward only: */

@@ -7,7 +7,7 @@ namespace seq {
 static int check_args(const taco_linear_attention_args *a) {
     SEQ_NEED(a, "args: null");
     if (int rc = check_dims(a->heads, a->heads, a->dim, a->dtype)) return rc;
-    SEQ_NEED(a->scale != 0.f && __builtin_fabsf(a->scale) < __builtin_inff(), "scale %g: finite and not 0", (double)a->scale);
+    SEQ_NEED(__builtin_fabsf(a->scale) >= 1.17549435e-38f && __builtin_fabsf(a->scale) < __builtin_inff(), "scale %g: finite and not 0 (nor below float32's normal range)", (double)a->scale);
     SEQ_NEED(a->n_sequences >= 0 && a->n_segments >= a->n_sequences, "%d segments of %d sequences", a->n_segments, a->n_sequences);
     SEQ_NEED((int64_t)a->n_sequences * a->heads <= 65535 || a->n_segments == a->n_sequences, "%d sequences of %d heads: at most 65535 in all where they are cut into segments",
              a->n_sequences, a->heads);

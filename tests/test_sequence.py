@@ -388,3 +388,10 @@ def test_an_output_that_requires_a_gradient_is_refused():
               lambda: s.linear_attention_step(x, x, x, Fake((2,)), Fake((4, 2, 32, 32)), out=out)):
         with pytest.raises(_lib.TacoError, match="out requires a gradient"):
             f()
+
+
+def test_a_scale_whose_inverse_is_infinite_is_refused(lib):
+    """the gradients of linear attention carry their states divided by it"""
+    for scale, code in ((1e-40, -1), (-1e-40, -1), (2.0 ** -126, 0), (-1.0, 0)):
+        for f in (lib.taco_linear_attention, lib.taco_linear_attention_backward):
+            assert f(C.byref(linear_args(scale=scale, n_segments=0, n_sequences=0)), None) == code
