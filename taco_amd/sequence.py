@@ -19,6 +19,7 @@ the graph, and capture a backward pass only while no eager autograd graph of the
 inside the capture, which it does not survive.
 """
 import ctypes as C
+import functools
 import math
 
 import numpy as np
@@ -351,8 +352,38 @@ def _empty(shape, total, dtype, device):
     return t
 
 
+class _OnceOnly(torch.autograd.Function):
+    """The last `count` tensors, as functions of those before them whose derivative is refused: gradients that were asked for with create_graph, which torch would
+    otherwise take for constants wherever the upstream gradient is one."""
+    @staticmethod
+    def forward(ctx, count, *tensors):
+        return tuple(t.clone() for t in tensors[-count:])
+
+    @staticmethod
+    def backward(ctx, *_):
+        raise _lib.TacoError("the sequence operators have no second derivative")
+
+
+def _first_derivative(f):
+    """of a Function's backward pass: it runs unrecorded, and what it returns cannot be differentiated again"""
+    @functools.wraps(f)
+    def backward(ctx, *upstream):
+        with torch.no_grad():
+            grads = f(ctx, *upstream)
+        if not torch.is_grad_enabled():
+            return grads
+        at = [i for i, g in enumerate(grads) if g is not None]
+        if at:
+            of = [t for t in (*ctx.saved_tensors, *upstream) if t is not None]
+            grads = list(grads)
+            for i, g in zip(at, _OnceOnly.apply(len(at), *of, *(grads[i] for i in at))):
+                grads[i] = g
+        return tuple(grads)
+    return backward
+
+
 def _attention_forward(q, k, v, seqs, causal, scale, out):
-    q, k, v = _usable(q), _usable(k), _usable(v)
+    """(q, k and v as _usable returned them)"""
     total, device = seqs.total, q.device
     o = _empty(q.shape, total, q.dtype, device) if out is None else out
     lse = _empty(q.shape[:2], total, torch.float32, device)
@@ -360,13 +391,13 @@ def _attention_forward(q, k, v, seqs, causal, scale, out):
         _written(out)
     if total:
         _launch_tiles(_attention_args(q, k, v, o, lse, seqs, causal, scale), seqs, device, False)
-    return q, k, v, o, lse
+    return o, lse
 
 
 class _Attention(torch.autograd.Function):
     @staticmethod
     def forward(ctx, q, k, v, seqs, causal, scale):
-        q, k, v, o, lse = _attention_forward(q, k, v, seqs, causal, scale, None)
+        o, lse = _attention_forward(q, k, v, seqs, causal, scale, None)
         ctx.save_for_backward(q, k, v, o, lse)
         ctx.rest = seqs, causal, scale
         ctx.mark_non_differentiable(lse)
@@ -374,7 +405,7 @@ class _Attention(torch.autograd.Function):
         return o, lse
 
     @staticmethod
-    @torch.autograd.function.once_differentiable
+    @_first_derivative
     def backward(ctx, d_o, _):
         if d_o is None:
             return (None,) * 6
@@ -417,7 +448,8 @@ def attention(q, k, v, sequences, causal=True, scale=None, return_lse=False, out
         if grad:
             raise ValueError("out= cannot be given where a gradient is recorded")
         _check_out(out, q)
-    o, lse = _Attention.apply(q, k, v, sequences, causal, scale) if grad else _attention_forward(q, k, v, sequences, causal, scale, out)[3:]
+    q, k, v = _usable(q), _usable(k), _usable(v)
+    o, lse = _Attention.apply(q, k, v, sequences, causal, scale) if grad else _attention_forward(q, k, v, sequences, causal, scale, out)
     return (o, lse) if return_lse else o
 
 
@@ -519,7 +551,7 @@ def _linear_workspace(a, seqs, backward, device):
 
 
 def _linear_forward(q, k, v, log_decay, state, seqs, scale):
-    q, k, v = _usable(q), _usable(k), _usable(v)
+    """(q, k and v as _usable returned them)"""
     o = _empty(q.shape, seqs.total, q.dtype, q.device)
     last = torch.empty((len(seqs), q.shape[1], q.shape[2], q.shape[2]), dtype=torch.float32, device=q.device)
     if not seqs.total:              # no token: the states stay as they are
@@ -530,20 +562,20 @@ def _linear_forward(q, k, v, log_decay, state, seqs, scale):
         ws = _linear_workspace(a, seqs, False, q.device)
         _call(load().taco_linear_attention, a, q.device)
         del ws
-    return q, k, v, o, last
+    return o, last
 
 
 class _Linear(torch.autograd.Function):
     @staticmethod
     def forward(ctx, q, k, v, log_decay, state, seqs, scale):
-        q, k, v, o, last = _linear_forward(q, k, v, log_decay, state, seqs, scale)
+        o, last = _linear_forward(q, k, v, log_decay, state, seqs, scale)
         ctx.save_for_backward(q, k, v, log_decay, state)
         ctx.rest = seqs, scale
         ctx.set_materialize_grads(False)
         return o, last
 
     @staticmethod
-    @torch.autograd.function.once_differentiable
+    @_first_derivative
     def backward(ctx, d_o, d_last):
         q, k, v, log_decay, state = ctx.saved_tensors
         seqs, scale = ctx.rest
@@ -592,9 +624,10 @@ def linear_attention(q, k, v, log_decay, sequences, state=None, scale=None):
             raise ValueError(f"state: float32 [{len(sequences)}, {H}, {d}, {d}] on {device} expected")
         state = state.contiguous()
     scale = _scale(scale, d, False)
+    q, k, v = _usable(q), _usable(k), _usable(v)
     if torch.is_grad_enabled() and any(t is not None and t.requires_grad for t in (q, k, v, state)):
         return _Linear.apply(q, k, v, log_decay, state, sequences, scale)
-    return _linear_forward(q, k, v, log_decay, state, sequences, scale)[3:]
+    return _linear_forward(q, k, v, log_decay, state, sequences, scale)
 
 
 _RESET_BYTES = {torch.bool: 1, torch.uint8: 1, torch.int32: 4, torch.int64: 8}

@@ -395,3 +395,35 @@ def test_a_scale_whose_inverse_is_infinite_is_refused(lib):
     for scale, code in ((1e-40, -1), (-1e-40, -1), (2.0 ** -126, 0), (-1.0, 0)):
         for f in (lib.taco_linear_attention, lib.taco_linear_attention_backward):
             assert f(C.byref(linear_args(scale=scale, n_segments=0, n_sequences=0)), None) == code
+
+
+@pytest.mark.parametrize("op", ["attention", "linear"])
+@pytest.mark.parametrize("strided", [False, True])
+def test_second_derivatives_are_refused(monkeypatch, op, strided):
+    """a gradient that was asked for with create_graph, in a loss of its own: not a constant, also where the upstream gradient is one (a sum's).  The kernels are left out here."""
+    s, seqs = sequence, sequence.Packed([3, 1], "cuda:0")
+    monkeypatch.setattr(s, "_check_rows", lambda what, q, *others: (torch.device("cuda:0"), 0))
+    monkeypatch.setattr(s, "_check_decay", lambda log_decay, heads, device: log_decay)
+    monkeypatch.setattr(s, "_launch_tiles", lambda a, seqs, device, backward: None)
+    monkeypatch.setattr(s, "_call", lambda f, a, device: None)
+    monkeypatch.setattr(s.Packed, "_segments", lambda self, work: (torch.zeros(2, 8), torch.zeros(3), 2))
+    leaf = [torch.randn(4, 2, 41 if strided else 32, requires_grad=True) for _ in range(3)]
+    x = [t[..., :32] for t in leaf]
+
+    def run():
+        return s.attention(*x, seqs) if op == "attention" else s.linear_attention(*x, torch.zeros(2), seqs)[0]
+    plain = torch.autograd.grad(run().sum(), leaf)
+    for i in range(3):
+        o = run()
+        g, = torch.autograd.grad(o.sum(), leaf[i], create_graph=True)
+        assert g.shape == plain[i].shape and g.requires_grad
+        loss = o.sum() + g.square().sum()
+        with pytest.raises(_lib.TacoError, match="second derivative"):
+            torch.autograd.grad(loss, leaf[i], retain_graph=True)
+        with pytest.raises(_lib.TacoError, match="second derivative"):
+            loss.backward()
+    for t in leaf:
+        t.grad = None
+    run().sum().backward(create_graph=True)
+    for t in leaf:
+        t.grad.zero_()

@@ -86,3 +86,24 @@ def test_attention_step_heads_before_rows():
     kp, vp = (torch.randn(1, 8, 1, d, generator=torch.Generator("cuda").manual_seed(i), device="cuda", dtype=torch.float16) for i in (2, 3))
     args = kp, vp, torch.zeros(B, 1, dtype=torch.int32, device="cuda"), torch.arange(B, device="cuda", dtype=torch.int32) % 9
     assert torch.equal(S().attention_step(q, None, None, *args), S().attention_step(q.contiguous(), None, None, *args))
+
+
+@pytest.mark.parametrize("op", ["attention", "linear"])
+def test_gradients_asked_for_with_create_graph(op):
+    """the same bits, and a second derivative is refused instead of left out (a gradient penalty)"""
+    leaf = [randn(50, 2, 41, seed=i).requires_grad_() for i in range(3)]       # (rows that are copied first)
+    state, decay, seqs = randn(2, 2, 40, 40).requires_grad_(), torch.full((2,), -0.1, device="cuda"), S().Packed([30, 20], "cuda:0")
+    x = [t[..., :40] for t in leaf]
+    of = leaf + [state] if op == "linear" else leaf
+
+    def out():
+        return S().attention(*x, seqs).sum() if op == "attention" else sum(t.sum() for t in S().linear_attention(*x, decay, seqs, state=state))
+    want = torch.autograd.grad(out(), of)
+    for i, t in enumerate(of):
+        o = out()
+        g, = torch.autograd.grad(o, t, create_graph=True)
+        assert torch.equal(g, want[i])
+        with pytest.raises(_lib.TacoError, match="second derivative"):
+            torch.autograd.grad(o + g.square().sum(), t)
+    out().backward(create_graph=True)
+    assert all(torch.equal(t.grad, w) for t, w in zip(of, want))
