@@ -69,9 +69,10 @@ int taco_attention_backward(const taco_attention_args *a, void *stream);
 /* ---- Attention of one new token per row over a paged cache, which the token joins.
  * Token t of row b lies in page table[b][t / page_size], slot t % page_size.  Row b's cache holds lengths[b] tokens before the call.  With k_new and
  * v_new the token becomes number lengths[b] (written into the cache) and is attended too; without (NULL), the cache is read as it is, and a row of
- * length 0 gets zeros.  lengths is not changed.  A page that several rows share may be read by all; the slot a token is written to must be one row's.
+ * length 0 gets zeros.  lengths is not changed.  A page that several rows share may be read by all; the slot a token is written to must be one row's, and named once.
  * A row whose length is negative or leaves no room in its table, or whose table names a page outside [0, num_pages) for a token that is read, gets
- * NaN in its output; nothing outside the buffers is read or written, and the rows beside it are not touched. */
+ * NaN in its output; nothing outside the buffers is read or written, and the rows beside it are not touched (its own token still joins the cache
+ * if that has a page and a slot). */
 typedef struct taco_attention_step_args {
     taco_seq_tensor q, o;               /* [rows][heads][dim]: token_stride = the row's */
     taco_seq_tensor k_new, v_new;       /* [rows][kv_heads][dim], or both NULL */

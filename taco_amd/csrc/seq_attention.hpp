@@ -27,8 +27,9 @@ __device__ __forceinline__ void locate(int block, int heads, int &tile, int &hea
     if (heads % 8 == 0) head = (head % 8) * (heads / 8) + head / 8;
 }
 
-// Wavefronts per SIMD that the registers are cut for: as many as do not spill.  Nothing else hides the latency of loads and of the chain of products, least
-// of all where a sequence is one tile.
+// Wavefronts per SIMD that the registers are cut for: as many as spill nothing, or little.  Nothing else hides the latency of loads and of the chain of products, least
+// of all where a sequence is one tile.  Cut for two, these spill at rows of 128 in 16 bits: the forward 15 to 17 registers, dQ 58, dK / dV 9 to 12.  Cut for one: float32
+// dQ of 128 in 32-row tiles 104, the forward there 29, the short gradients of 96 29; fp16's short gradients of 128 12, dK / dV of 64 2.
 template <typename T, int DP, int NW> constexpr int waves_forward = sizeof(T) == 4 ? (DP == 32 ? 2 : 1) : DP == 32 ? 4 : DP == 64 || NW == 4 ? 2 : 1;
 template <typename T, int DP, int NW> constexpr int waves_dq = sizeof(T) == 4 ? (DP == 32 ? 2 : 1) : DP <= 64 || NW == 4 ? 2 : 1;
 template <typename T, int DP> constexpr int waves_dkv = sizeof(T) == 4 ? (DP == 32 ? 2 : 1) : DP <= 64 ? 2 : 1;
@@ -73,7 +74,7 @@ template <typename T, int DP> __device__ __forceinline__ void add_columns(const 
 // Bound by LDS (32 KB a wavefront and tile for 1 024 clocks of matrix work) and the exponentials, which only the second wavefront of the SIMD hides.  One
 // sequence of 16 384 tokens, 16 heads of 128 over 4, bf16: 1.10 to 1.13 ms, 975 to 1 000 TFLOP/s (a library product of 8 192^3: 1 138); with the masks and the test for
 // NaN in the one loop, and what that spilled, 9.3 ms.  24 sequences of up to 2 048: 0.25 ms, 627: tiles of 12 turns on average, whose first loads and
-// half-hidden tiles nothing covers.
+// half-hidden tiles nothing covers.  fp16, with its lift: 1.28 ms for the one of 16 384 (1.26 without).
 template <typename T, int DP, int NW>
 __global__ __launch_bounds__(64 * NW, (waves_forward<T, DP, NW>)) void attention_kernel(AttentionParams p) {
     typedef Tile<T, DP> tile;
@@ -219,7 +220,8 @@ __global__ __launch_bounds__(64 * NW, (waves_forward<T, DP, NW>)) void attention
 // products for five), because neither then needs an atomic or a float32 copy of a gradient.
 // A query that sees few keys has gradients that are small differences of dP and delta, and o as it was rounded would set their error.  Where all its keys
 // lie in one tile, delta is the sum of P dP over that tile instead, in float32 (from o, dq and dk of sequences of two tokens were 2.3 roundings off, now 1.4).
-// Six sequences of up to 4 096, 16 heads of 128 over 4, bf16: 0.41 ms, 740 TFLOP/s of its three products; bound as the forward.
+// Six sequences of up to 4 096, 16 heads of 128 over 4, bf16: 0.41 ms, 740 TFLOP/s of its three products (fp16 0.45); bound as the forward, and by what it spills
+// (243 MB written, 65 of them dQ).
 template <typename T, int DP, int NW>
 __global__ __launch_bounds__(64 * NW, (waves_dq<T, DP, NW>)) void attention_dq_kernel(AttentionParams p) {
     typedef Tile<T, DP> tile;
@@ -535,7 +537,7 @@ __global__ __launch_bounds__(64 * NW, (waves_dkv<T, DP>)) void attention_dkv_ker
 // The same for 128 keys of 16 bits and rows of 128, where the operands and sums of 32 keys leave room for one wavefront on a SIMD only, and nothing to hide its
 // waits behind.  K and V stay in LDS instead, and two wavefronts own the same 32 keys: one takes the first 32 queries of each tile, one the others; their
 // sums meet in LDS at the end.  Six sequences of up to 4 096 tokens, 16 heads over 4, bf16: 0.57 ms, 710 TFLOP/s of its four products (0.70 ms with one
-// wavefront); LDS (48 KB a wavefront and tile for 1 024 clocks of matrix work) is the nearer bound.
+// wavefront); LDS (48 KB a wavefront and tile for 1 024 clocks of matrix work) is the nearer bound.  fp16 0.61 ms.
 template <typename T, int DP> constexpr bool keys_in_lds = sizeof(T) == 2 && DP == 128;
 template <typename T, int DP>
 __global__ __launch_bounds__(512, 2) void attention_dkv_pair_kernel(AttentionParams p) {

@@ -98,7 +98,7 @@ template <typename T, int N> __device__ __forceinline__ void lift(f32x16 &x, flo
         x *= f;
     }
 }
-// A weight of a softmax is at most 1 (and its rounding more): always lifted by 2^15, the sum lowered by as much
+// A softmax's weight is at most 1 (a rounding more as it is computed): always lifted by 2^15, and the sum lowered by as much
 template <typename T> constexpr float LIFT = narrow<T> ? 15.f : 0.f;
 template <typename T> constexpr float WEIGHT = narrow<T> ? 32768.f : 1.f;
 template <typename T> constexpr float lift_start = narrow<T> ? 18446744073709551616.f : 1.f;

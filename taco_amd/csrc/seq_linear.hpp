@@ -36,7 +36,7 @@ __device__ __forceinline__ float decay2(const float *log_decay, int head) {
 
 // acc[b] += K^T (V * tail), C tokens' part of the state, from row0.  tail decays per token, so V * tail has float32's 24 bits; it goes through the 16-bit product in
 // parts that add up to it, and the state stays as exact as float32 sums: bf16 in three parts of 8 bits; fp16 in two of 11 (the second scaled by 2^11, with
-// a sum of its own, so that small values do not fall below fp16's range).
+// a sum of its own: what is lost of a value is below 2^-36, as much as float32 would lose of values of 2^-12 and more).
 template <typename T, int DP, int C> __device__ __forceinline__ void add_outer(const char *lds_k, const char *lds_v, const float *tail, int row0, int col0, f32x16 (&acc)[DP / 32], int lane) {
     typedef Tile<T, DP> tile;
     constexpr int E = C / 16, PARTS = sizeof(T) == 4 ? 1 : __is_same(T, f16) ? 2 : 3;
@@ -94,7 +94,7 @@ template <typename T, int DP, int C> __device__ __forceinline__ void add_outer(c
 // P and S are rounded to the inputs' type for their products, the state itself never is.  In float16 a column of S that does not fit the type is lifted by a power of two (a
 // gradient's state is divided by the scale: 5 800 is past 65 504 there with heads of 128).
 // 28 700 tokens in 6 sequences, 16 heads of 128, bf16: 0.15 ms for the outputs, 3.1 TB/s (without the outputs' products 0.10: the rest is their latency), 0.07 for
-// the segments' own states, 0.01 for joining them: 0.21 ms in all.  With one wavefront for both parts and its spills it took 0.58.
+// the segments' own states, 0.01 for joining them: 0.21 ms in all.  With one wavefront for both parts and its spills it took 0.58.  fp16 pays 1 to 5 % for looking at the states' and weights' range.
 // STATES: only the state that the segment makes from nothing, for `carry`; there are fewer of these than CUs, so each chunk is shared out to QB keepers, 32
 // tokens each, whose sums meet in LDS at the end.
 template <typename T> constexpr int chunk_of = sizeof(T) == 4 ? 32 : 64;        // (float32: the tiles and the state's copy have to fit 160 KB of LDS)

@@ -32,7 +32,7 @@ ABI_VERSION = 2
 EXPORTS = ["taco_sequence_abi_version", "taco_sequence_source_hash", "taco_sequence_last_error", "taco_attention", "taco_attention_backward",
            "taco_attention_step_workspace_bytes", "taco_attention_step", "taco_linear_attention_workspace_bytes", "taco_linear_attention",
            "taco_linear_attention_backward", "taco_linear_attention_step"]
-_FEW_SHORT = 1024       # workgroups of sequences of at most 64 tokens (four a CU) that still join the launch of the 128-row tiles
+_FEW_SHORT = 1024       # workgroups of sequences of at most 64 tokens (four a CU) that still join the launch of the 128-row tiles (measured in Packed._tiles, on one shape)
 _DTYPES = {torch.float32: 0, torch.float16: 1, torch.bfloat16: 2}
 
 
@@ -169,7 +169,8 @@ def _scale(scale, dim, positive):
     if scale is None:
         return 1.0 / math.sqrt(dim)
     if isinstance(scale, torch.Tensor):
-        _no_tangent("the scale", scale)
+        if forward_ad._current_level >= 0:
+            _no_tangent("the scale", scale)
         if scale.requires_grad and torch.is_grad_enabled():
             raise _lib.TacoError("the scale has no gradient: give its value, or multiply q by it")
     scale = float(scale)
@@ -185,7 +186,7 @@ def _no_grad(tensors, what):
 
 def _no_tangent(what, *tensors):
     """a dual tensor does not require a gradient: without this its tangent would be lost, and the result count as constant"""
-    if forward_ad._current_level >= 0 and any(t is not None and forward_ad.unpack_dual(t).tangent is not None for t in tensors):
+    if any(t is not None and forward_ad.unpack_dual(t).tangent is not None for t in tensors):
         raise _lib.TacoError(f"{what} has no forward-mode derivative")
 
 
@@ -288,7 +289,8 @@ class Packed:
         idle; each cut costs a second reading of its k and v and the state's way through memory and back.  Of some lengths (at least 256 tokens; sequences
         are cut into equal pieces) the one with the least estimate is taken, in tokens of a CU's time: the longest segment if all run at once, else a CU's
         share and half the longest; a third for a token that is read again; 160 for a state (six sequences of 28 700 tokens, 16 heads: 213 us in 15
-        segments, 241 in 34)."""
+        segments, 241 in 34).  Both weights come from that one shape, bf16 heads of 128; a state's goes with the square of the head size and neither that nor the type
+        enters: elsewhere the estimate chooses a working cut, not always the best."""
         got = self._lists.get(("segments", work))
         if got is not None:
             return self._kept(("segments", work), None)
@@ -434,7 +436,8 @@ def attention(q, k, v, sequences, causal=True, scale=None, return_lse=False, out
     A token that is hidden has no influence, even where it holds NaN or infinities, forward and backward; a token whose scores are all -inf gets zeros.  Rows behind the last sequence: zero in new
     tensors and in gradients, untouched in `out` (which cannot be given where a gradient is recorded, and must not overlap q, k or v).
     Strides: any, as long as `dim` is contiguous and rows are multiples of 16 bytes; other layouts are copied first."""
-    _no_tangent("attention", q, k, v, out)
+    if forward_ad._current_level >= 0:
+        _no_tangent("attention", q, k, v, out)
     device, _ = _check_rows("attention", q, ("k", k), ("v", v))
     (T, H, d), Hk = q.shape, k.shape[1]
     if k.shape != v.shape or k.shape[0] != T:
@@ -478,11 +481,13 @@ def attention_step(q, k, v, k_pages, v_pages, page_table, lengths, scale=None, o
     so a [pages, kv_heads, page_size, dim] cache is passed transposed); page_table int32 [rows, width]; lengths int32 [rows]: tokens in each row's cache
     BEFORE the call.  Token t of row b is page page_table[b, t // page_size], slot t % page_size.  The new token is written as token lengths[b] and
     attended too; lengths itself is the caller's to advance.  k = v = None: the cache is read as it is (a row of length 0 gives zeros).
-    Rows may share pages that they only read.  A row whose length is negative or has no room in its table, or that reads a page number outside the cache,
-    gives NaN; nothing else is touched.  -> [rows, heads, dim] (`out` if given, which must not overlap the inputs).  No gradient."""
+    Rows may share pages that they only read; the slot a token is written to has to be named once, by one row, and rows that take no part get a length of -1.
+    A row whose length is negative or has no room in its table, or that reads a page number outside the cache, gives NaN; what other rows hold is not touched
+    (its own token still joins the cache if that has a page and a slot).  -> [rows, heads, dim] (`out` if given, which must not overlap the inputs).  No gradient."""
     if (k is None) != (v is None):
         raise ValueError("k and v: both or none")
-    _no_tangent("attention_step", q, k, v, k_pages, v_pages, out)
+    if forward_ad._current_level >= 0:
+        _no_tangent("attention_step", q, k, v, k_pages, v_pages, out)
     device, code = _check_rows("attention_step", q) if k is None else _check_rows("attention_step", q, ("k", k), ("v", v))
     B, H, d = q.shape
     ks, vs = _check_pages("k_pages", k_pages, q), _check_pages("v_pages", v_pages, q)
@@ -612,7 +617,8 @@ def linear_attention(q, k, v, log_decay, sequences, state=None, scale=None):
     scale: 1 / sqrt(dim).  -> (o [T, heads, dim], the states behind the last tokens, float32).  Gradients for q, k, v and state.
     A later token has no influence on an earlier output, even where it holds NaN or infinities; a value that is not finite makes the outputs of its own chunk of
     64 tokens and the state NaN.  In float16 a growth (log_decay > 0) must leave v exp(64 log_decay) inside the type's range."""
-    _no_tangent("linear_attention", q, k, v, log_decay, state)
+    if forward_ad._current_level >= 0:
+        _no_tangent("linear_attention", q, k, v, log_decay, state)
     device, _ = _check_rows("linear_attention", q, ("k", k), ("v", v))
     if not q.shape == k.shape == v.shape or not q.shape[1]:
         raise ValueError(f"q {tuple(q.shape)}, k {tuple(k.shape)}, v {tuple(v.shape)}: alike expected")
@@ -637,7 +643,8 @@ def linear_attention_step(q, k, v, log_decay, state, reset=None, scale=None, out
     """One token per row of linear_attention: q, k, v [rows, heads, dim]; state float32 [rows, heads, dim, dim], contiguous, updated in place; reset [rows] (bool,
     uint8, int32 or int64, e.g. env.reset_buf): rows that begin anew, whatever their state holds.  -> [rows, heads, dim] (`out` if given, which must not
     overlap the inputs).  No gradient."""
-    _no_tangent("linear_attention_step", q, k, v, log_decay, state, out)
+    if forward_ad._current_level >= 0:
+        _no_tangent("linear_attention_step", q, k, v, log_decay, state, out)
     device, code = _check_rows("linear_attention_step", q, ("k", k), ("v", v))
     shape = q.shape
     B, H, d = shape
